@@ -268,6 +268,51 @@ int lb_attention_decode_noalloc(void* stream, uint64_t q, uint64_t k_new, uint64
                                 uint64_t k_norm_w, uint64_t k_cache, uint64_t v_cache, uint64_t out, int pos, int HQ,
                                 int HKV, int in_is_f32, int rot_dims, float rope_theta, float eps, char* err, size_t errlen);
 
+/* ---- a batch of sequences over a 4-bit cache -------------------------------------------
+ * No counterpart in the reference, whose caches are bf16 and hold one sequence.  For a host that decodes several sequences at a time: projections by
+ * lb_gemm_int4, then lb_kv4_append and lb_kv4_attention per layer, tokens by lb_verify_drafts.
+ *
+ * The cache: a caller's buffer of lb_kv4_bytes bytes (16-byte aligned), 4.5 bits a value, which needs no initial values: rows are read only after they were
+ * written.  Per sequence and KV head, rows in blocks of 16, S = dim / 64 groups of features:
+ *   u8 keys [2][S][8][32], u8 values [S][8][16][4], then fp16 (scale, lowest) of the keys [S][16][2] and of the values [S][16][2];
+ * row r of a block has its keys at half (r / 2) % 2, place 2 (r / 4) + r % 2; a byte holds two neighbouring features, the lower one in its low half.  A code c stands
+ * for lowest + scale * c: lowest is the minimum of the row's group of 64 features, scale = (maximum - lowest) / 15, both rounded to fp32 and then to fp16 (values
+ * beyond fp16's range are cut off there), c the nearest code in 64-bit arithmetic, halves to the even one.  A group with a NaN or an infinity stands for NaN.
+ *
+ * The batch: token rows starts[r] .. starts[r+1]-1 are the new tokens of request r, which is sequence seqs[r] with pos[r] rows in the cache before the call; the i-th of
+ * them is (or becomes) row pos[r] + i.  seqs = 0: request r is sequence r; starts = 0: one token each.  The arrays lie on the device and are read when the
+ * kernel runs, so a captured graph takes new ones.  A request whose rows end behind max_ctx is left out whole, status word 0x1005; one that names token rows or a
+ * sequence that are not there (or more than max_new tokens) likewise, 0x1006.  starts is ascending; token rows behind the last request's are left as they were.
+ * A request without tokens does nothing. */
+enum { LB_IN_BF16 = 0, LB_IN_F32 = 1, LB_IN_F16 = 2 }; /* element types */
+enum { LB_KV4_MAX_REQS = 256, LB_KV4_MAX_NEW = 16 };
+typedef struct {
+    uint64_t data;
+    int32_t n_seqs;   /* 1 .. 2^20 - 1 */
+    int32_t max_ctx;  /* rows per sequence: a multiple of 16, up to 2^20 */
+    int32_t kv_heads; /* 1 .. 32 */
+    int32_t dim;      /* 64, 128 or 256 */
+} lb_kv4_cache;
+typedef struct {
+    uint64_t seqs, pos, starts; /* i32 [n_reqs], [n_reqs], [n_reqs + 1] */
+    int32_t n_reqs;             /* 1 .. LB_KV4_MAX_REQS */
+    int32_t rows;               /* token rows that the call's tensors have */
+} lb_kv4_batch;
+size_t lb_kv4_bytes(int n_seqs, int max_ctx, int kv_heads, int dim); /* 0: not a shape of these calls */
+/* New rows into the cache.  k, v: element type `type`, heads next to each other, token rows `stride` elements apart (0: kv_heads * dim).  Keys are normalised
+ * per head (k_norm_w bf16 [dim]; 0: not) and their first rot_dims features rotated in neighbouring pairs by position, as lb_attention_decode does it.  Where two requests
+ * bring the same row of the same sequence, the later request's stays. */
+int lb_kv4_append(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t k, uint64_t v, int64_t stride, int type, uint64_t k_norm_w,
+                  int rot_dims, float rope_theta, float eps);
+/* The rows that the batch names, as values: k_out, v_out [rows, kv_heads, dim] of element type `type` (one rounding) */
+int lb_kv4_read(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t k_out, uint64_t v_out, int type);
+/* Attention of the batch's new tokens, whose rows are in the cache: token i of request r sees rows 0 .. pos[r] + i.
+ * q and gate (0: none): element type `type`, head h of token row j at j * row_stride + h * head_stride elements (row_stride 0: n_heads * head_stride, head_stride 0: dim); q is
+ * normalised per head (q_norm_w; 0: not) and rotated like the keys, then rounded to fp16; the result is multiplied by sigmoid(gate).  n_heads: 1 to 16 times
+ * kv_heads.  max_new: the most tokens a request of the batch has, 1 .. LB_KV4_MAX_NEW.  out fp16 [rows, n_heads, dim], what lb_gemm_int4 takes. */
+int lb_kv4_attention(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t q, uint64_t gate, int64_t row_stride, int64_t head_stride, int type,
+                     uint64_t q_norm_w, uint64_t out_f16, int n_heads, int max_new, int rot_dims, float rope_theta, float eps);
+
 /* ---- small kernels ---------------------------------------------------------------------
  * rmsnorm: replaces launch_norm (src/launcher.s:1101-1219, inference/reduce.ls:21-147);
  * argmax: replaces the CPU argmax loop (src/launcher.s:962-1073, inference/reduce.ls:214-313);

@@ -25,6 +25,7 @@ LB_ERR_DEVICE_WAIT, LB_ERR_IO, LB_ERR_NOMEM, LB_ERR_STATE = 5, 6, 7, 8
 
 GEMV_X_F32, GEMV_Y_F32, GEMV_Y_ACCUM, GEMV_Y_SWIGLU = 1, 2, 4, 8
 GEMM_MMA_SYNC, GEMM_TCGEN05 = 16, 32
+IN_BF16, IN_F32, IN_F16 = 0, 1, 2
 X_F16, X_F32, X_F32_RMSNORM, X_F32_HEADNORM_SILU = 0, 1, 2, 3
 Y_F16, Y_F32, Y_F32_ACCUM, Y_SWIGLU_F16 = 0, 1, 2, 3
 
@@ -126,8 +127,28 @@ def lib() -> C.CDLL:
     sig("lb_argmax", i32, vp, u64, i32, u64)
     sig("lb_embed", i32, vp, u64, u64, u64, i32)
     sig("lb_sample_topk", i32, vp, u64, i32, f32, i32, u64, u64, u64, u64, u64)
+    KC, KB, i64 = P(Kv4Cache), P(Kv4Batch), C.c_int64
+    sig("lb_kv4_bytes", sz, i32, i32, i32, i32)
+    sig("lb_kv4_append", i32, vp, KC, KB, u64, u64, i64, i32, u64, i32, f32, f32)
+    sig("lb_kv4_read", i32, vp, KC, KB, u64, u64, i32)
+    sig("lb_kv4_attention", i32, vp, KC, KB, u64, u64, i64, i64, i32, u64, u64, i32, i32, i32, f32, f32)
     _lib = L
     return L
+
+
+class Kv4Cache(C.Structure):
+    """lb_kv4_cache: the 4-bit cache of n_seqs sequences at device address `data` (kv4_bytes bytes)"""
+    _fields_ = [("data", C.c_uint64)] + [(n, C.c_int32) for n in ("n_seqs", "max_ctx", "kv_heads", "dim")]
+
+
+class Kv4Batch(C.Structure):
+    """lb_kv4_batch: device addresses of seqs, pos, starts (0: see the header), requests, token rows"""
+    _fields_ = [(n, C.c_uint64) for n in ("seqs", "pos", "starts")] + [(n, C.c_int32) for n in ("n_reqs", "rows")]
+
+
+def kv4_bytes(n_seqs: int, max_ctx: int, kv_heads: int, dim: int) -> int:
+    """bytes of a 4-bit cache, or 0 for a shape that there is none for"""
+    return lib().lb_kv4_bytes(n_seqs, max_ctx, kv_heads, dim)
 
 
 class GemvOp(C.Structure):
@@ -401,6 +422,19 @@ class Context:
                                               q_norm_w.ptr if q_norm_w else 0, k_norm_w.ptr if k_norm_w else 0,
                                               k_cache.ptr, v_cache.ptr, out.ptr, pos, HQ, HKV, 1 if in_is_f32 else 0,
                                               rot_dims, rope_theta, eps))
+
+    def kv4_append(self, cache, batch, k, v, stride=0, in_type=IN_BF16, k_norm_w=None, rot_dims=64, rope_theta=1e7, eps=1e-6):
+        """new key and value rows of a batch into its 4-bit cache"""
+        self._check(lib().lb_kv4_append(self.h, C.byref(cache), C.byref(batch), k.ptr, v.ptr, stride, in_type, k_norm_w.ptr if k_norm_w else 0, rot_dims, rope_theta, eps))
+
+    def kv4_read(self, cache, batch, k_out, v_out, out_type=IN_F32):
+        """the rows that a batch names, as the values that the cache stands for"""
+        self._check(lib().lb_kv4_read(self.h, C.byref(cache), C.byref(batch), k_out.ptr, v_out.ptr, out_type))
+
+    def kv4_attention(self, cache, batch, q, gate, row_stride, head_stride, in_type, q_norm_w, out, n_heads, max_new=1, rot_dims=64, rope_theta=1e7, eps=1e-6):
+        """attention of a batch's new tokens, whose rows are in the cache; out fp16 [rows, n_heads, dim]"""
+        self._check(lib().lb_kv4_attention(self.h, C.byref(cache), C.byref(batch), q.ptr, gate.ptr if gate else 0, row_stride, head_stride, in_type,
+                                           q_norm_w.ptr if q_norm_w else 0, out.ptr, n_heads, max_new, rot_dims, rope_theta, eps))
 
     def rmsnorm(self, x, res, w, y, sum_out, rows, D, eps=1e-6, one_plus_w=True):
         self._check(lib().lb_rmsnorm(self.h, x.ptr, res.ptr if res else 0, w.ptr, y.ptr, sum_out.ptr if sum_out else 0,

@@ -129,7 +129,7 @@ static int load_cubin(lb_ctx* c, const char* dir, const char* file) {
 
 static const char* const k_cubins[] = {"gemv.cubin", "chain.cubin", "batched.cubin", "batched_tc.cubin", "batched_ring.cubin", "deltanet.cubin", "attention.cubin", "attention_mma.cubin", "small.cubin", "comm.cubin", "prefill.cubin",
                                        "rows_gemv.cubin", "dense_gemm.cubin", "window_attention.cubin", "decay_attention.cubin",
-                                       "latent_attention.cubin", "ssm.cubin", "ssm_tc.cubin"};
+                                       "latent_attention.cubin", "ssm.cubin", "ssm_tc.cubin", "kv4_cache.cubin", "kv4_attention.cubin"};
 
 LB_API int lb_init(int device, const char* kernel_dir, lb_ctx** out) { return lb_init_images(device, kernel_dir, NULL, out); }
 
@@ -205,6 +205,11 @@ LB_API int lb_init_images(int device, const char* kernel_dir, const char* images
     c->attn_scratch_bytes = (size_t)8 * 64 * 8 * 260 * sizeof(float) + 256;
     LB_CU(c, lb_drv.MemAlloc(&c->attn_scratch, c->attn_scratch_bytes));
     LB_CU(c, lb_drv.MemsetD8Async(c->attn_scratch, 0, c->attn_scratch_bytes, c->stream));
+    if (c->fn[LBK_kv4_attn_256_1]) {
+        const size_t recs = (size_t)2 * 2 * c->sm_count * LB_KV4_COLS(1) * LB_KV4_REC(256) * sizeof(float); /* two a CTA; half the CTAs have twice the columns */
+        LB_CU(c, lb_drv.MemAlloc(&c->kv4_records, recs + 2 * (size_t)c->sm_count * sizeof(lb_kv4_join)));
+        c->kv4_joins = c->kv4_records + recs;
+    }
     LB_CU(c, lb_drv.MemAlloc(&c->chain_mail, (size_t)LB_CHAIN_MAX_OPS * LB_CHAIN_MAIL_WORDS * 8));
     LB_CU(c, lb_drv.MemsetD8Async(c->chain_mail, 0, (size_t)LB_CHAIN_MAX_OPS * LB_CHAIN_MAIL_WORDS * 8, c->stream));
     c->chain_mailbox = 1;
@@ -228,6 +233,7 @@ LB_API void lb_destroy(lb_ctx* c) {
         if (c->gemv_partial) lb_drv.MemFree(c->gemv_partial);
         if (c->gemv_counters) lb_drv.MemFree(c->gemv_counters);
         if (c->attn_scratch) lb_drv.MemFree(c->attn_scratch);
+        if (c->kv4_records) lb_drv.MemFree(c->kv4_records);
         if (c->dev_status) lb_drv.MemFree(c->dev_status);
         if (c->chain_mail) lb_drv.MemFree(c->chain_mail);
         if (c->flush_buf) lb_drv.MemFree(c->flush_buf);

@@ -198,6 +198,21 @@ int lb_driver_load(char* err, size_t errlen); /* LB_OK or LB_ERR_NO_DRIVER */
     X(ssm_tc)                         \
     X(ssm_tc_local)                   \
     X(ssm_finish)                     \
+    X(kv4_append_64)                  \
+    X(kv4_append_128)                 \
+    X(kv4_append_256)                 \
+    X(kv4_read_64)                    \
+    X(kv4_read_128)                   \
+    X(kv4_read_256)                   \
+    X(kv4_attn_64_1)                  \
+    X(kv4_attn_128_1)                 \
+    X(kv4_attn_256_1)                 \
+    X(kv4_attn_64_2)                  \
+    X(kv4_attn_128_2)                 \
+    X(kv4_attn_256_2)                 \
+    X(kv4_merge_64)                   \
+    X(kv4_merge_128)                  \
+    X(kv4_merge_256)                  \
     X(l2_flush)
 
 enum {
@@ -228,6 +243,8 @@ struct lb_ctx {
     CUdeviceptr gemv_counters; /* u32 per column tile, self-resetting */
     CUdeviceptr attn_scratch;  /* split-KV partials */
     size_t attn_scratch_bytes;
+    CUdeviceptr kv4_records;   /* partial results of the batch attention, then its joins; made with the context when its kernels are loaded */
+    CUdeviceptr kv4_joins;
     CUdeviceptr dev_status; /* u32 words written by bounded device-side waits */
     CUdeviceptr flush_buf;  /* L2 flush target */
     size_t flush_bytes;

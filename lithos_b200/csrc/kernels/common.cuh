@@ -13,6 +13,7 @@
 #define LB_DEV_TIMEOUT_PEER 0x1003u    // gave up waiting for a peer GPU's flag
 #define LB_DEV_TIMEOUT_COUNTER 0x1004u // gave up waiting on a split counter
 #define LB_DEV_POS_RANGE 0x1005u       // the decode position lies outside the KV cache: nothing was read or written
+#define LB_DEV_BATCH 0x1006u           // a request of a batch names token rows or a sequence that are not there: the request is left out
 // batched_tc.cu: a stage's products never completed; the last products never completed; a stage was never filled
 #define TC_FAIL_FREE 0x1101u
 #define TC_FAIL_DONE 0x1102u
@@ -27,6 +28,8 @@
 #define AC_FAIL_SCORES 0x1303u
 // batched_ring.cu: a slot was never filled
 #define RG_FAIL_FULL 0x1401u
+// kv4_attention.cu: a tile of the cache never landed
+#define KV_FAIL_FULL 0x1601u
 // ssm_tc.cu: a copy or a product never completed
 #define ST_FAIL 0x1501u
 

@@ -554,4 +554,56 @@ typedef struct {
     int32_t* pos;
 } lb_tp_argmax_params;
 
+/* ---- 4-bit KV cache of several sequences (kv4_cache.cu, kv4_attention.cu) ---------------------------------
+ * One record per sequence, KV head and 16 rows: LB_KV4_BLOCK(D) bytes, see kv4.cuh */
+#define LB_KV4_BLOCK(D) (18 * (D))
+#define LB_KV4_REQS 256   /* requests of a batch */
+#define LB_KV4_NEW 16     /* new tokens of a request in an attention call */
+#define LB_KV4_TILE 128   /* rows of a tile: the unit of work of the attention */
+typedef struct {
+    unsigned char* cache;
+    const int32_t* seqs;   /* [n_reqs] sequence of every request; NULL: request r is sequence r */
+    const int32_t* pos;    /* [n_reqs] rows in the cache before the call */
+    const int32_t* starts; /* [n_reqs + 1] first token row of every request; NULL: one token each */
+    uint32_t* status;
+    int32_t n_seqs, max_ctx, HKV, n_reqs, rows;
+    int32_t max_new;       /* most new tokens of a request (append, read: rows) */
+} lb_kv4_view;
+typedef struct {
+    lb_kv4_view b;
+    const void* k;          /* append: token row j's keys at k + j * stride elements, heads packed; read: out [rows, HKV, D] */
+    const void* v;
+    const uint16_t* norm_w; /* bf16 [D] or NULL */
+    int64_t stride;
+    int32_t D, type, rot_dims, wide; /* wide: rows may be read 16 bytes at a time */
+    double eps;
+    double freq[128];
+} lb_kv4_rows_params;
+#define LB_KV4_REC(D) ((D) + 4) /* floats of a column's record: D sums, maximum, sum, pad */
+typedef struct {               /* what a CTA's first item has to do with the CTA before it */
+    int32_t first, last;       /* contributors of the item, where the CTA before is the first of them; first < 0: nothing to merge */
+    int32_t row0, kv, col0, cols; /* the request's first token row; the item's columns col0.. (token * G + head) */
+    int32_t pad[2];
+} lb_kv4_join;
+typedef struct {
+    lb_kv4_view b;
+    const void* q;
+    const void* gate;       /* NULL: none */
+    const uint16_t* norm_w; /* bf16 [D] or NULL */
+    uint16_t* out;          /* fp16 [rows, HQ, D] */
+    float* records;         /* [CTAs][2][columns][LB_KV4_REC(D)] */
+    lb_kv4_join* joins;     /* [CTAs] */
+    int64_t row_stride, head_stride; /* of q and gate, elements */
+    int32_t HQ, type, rot_dims, wide;
+    float eps;
+    int32_t pad_;
+    double freq[128];
+} lb_kv4_attn_params;
+/* rings of the attention kernel: two CTAs per SM of 16 columns, or one of 32 */
+#define LB_KV4_STAGES(D, MT) ((D) == 256 ? ((MT) == 1 ? 2 : 4) : (D) == 128 ? ((MT) == 1 ? 4 : 6) : 6)
+#define LB_KV4_CTAS(MT) ((MT) == 1 ? 2 : 1) /* per SM */
+#define LB_KV4_COLS(MT) (16 * (MT))
+/* ring, queries, probabilities, the rest */
+#define LB_KV4_SMEM(D, MT) (LB_KV4_STAGES(D, MT) * 8 * LB_KV4_BLOCK(D) + (MT) * (D) * 32 + (MT) * (D) * 64 + 6 * 1024 + (MT) * 4 * 1024)
+
 #endif
