@@ -206,7 +206,11 @@ LB_API int lb_init_images(int device, const char* kernel_dir, const char* images
     LB_CU(c, lb_drv.MemAlloc(&c->attn_scratch, c->attn_scratch_bytes));
     LB_CU(c, lb_drv.MemsetD8Async(c->attn_scratch, 0, c->attn_scratch_bytes, c->stream));
     if (c->fn[LBK_kv4_attn_256_1]) {
-        const size_t recs = (size_t)2 * 2 * c->sm_count * LB_KV4_COLS(1) * LB_KV4_REC(256) * sizeof(float); /* two a CTA; half the CTAs have twice the columns */
+        size_t recs = 0; /* two a CTA */
+        for (int mt = 1; mt <= 4; mt *= 2) {
+            const size_t r = (size_t)2 * LB_KV4_CTAS(128, mt) * c->sm_count * LB_KV4_COLS(mt) * LB_KV4_REC(256) * sizeof(float);
+            if (r > recs) recs = r;
+        }
         LB_CU(c, lb_drv.MemAlloc(&c->kv4_records, recs + 2 * (size_t)c->sm_count * sizeof(lb_kv4_join)));
         c->kv4_joins = c->kv4_records + recs;
     }

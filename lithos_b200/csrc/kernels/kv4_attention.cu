@@ -1,13 +1,15 @@
 // Grouped-query attention of a batch's new tokens over the 4-bit KV cache (layout: kv4.cuh).
 //   out[j, h] = sum_t p_t v_t * sigmoid(gate[j, h]),  p = softmax over the rows t <= position of token j of  q[j, h] . k_t / sqrt(D),
 // q normalised and rotated as the decode attention does it.  The columns of an item (a request's KV head) are its new tokens times the query heads that share the
-// head; they are the 16 rows of the products (MT times 16), the cache's rows their other side.
+// head; 8 MT of them are taken at a time.
 //   * The codes are the products' operands as they are: four bits in the low end of a half are the subnormal c 2^-24, four bits above them c 2^-20, and the tensor cores
-//     take subnormals exactly.  A word of 8 codes costs a shift and four ANDs, no conversion; the 2^4 between neighbours is taken out of the query (keys) and of the sums
-//     (values).  scores = sum over groups of scale_t (q . c_t) + lowest_t sum(q); read-out = sum of (p_t scale_t) c_t + (p_t lowest_t), the second terms in fp32.
-//   * q goes in as fp16, a row scaled by a power of two to [2^13, 2^14) at its largest: 11 bits, as a fp16 projection gives them.  p scale goes in as fp16 too, scaled by a
-//     power of two per group and slice of the cache (its largest scale so far becomes [2^13, 2^14)), so that weights keep their 11 bits down to 2^-27 of the largest.
-//     Scores, running maxima, sums and read-outs are fp32; the output is fp16, what lb_gemm_int4 takes.
+//     take subnormals exactly, at their full rate.  A word of 8 codes costs a shift and four ANDs, no conversion; the 2^4 between neighbours is taken out of the query
+//     (keys) and of the sums (values).  scores = sum over groups of scale_t (q . c_t) + lowest_t sum(q); read-out = sum of (p_t scale_t) c_t + p_t lowest_t.
+//   * q and p scale go in as two fp16 terms, the leading one in rows 0..7 of a product and what it leaves in rows 8..15: 22 bits of each, for the price of rows that a
+//     group of up to 8 columns would leave empty.  A query is scaled by a power of two to [2^13, 2^14) at its largest; p (2^14 at the maximum) times scale by one per group, the
+//     largest scale so far becoming [1/2, 1): weights keep their bits down to 2^-27 of the largest.  Scores, maxima, sums and read-outs are fp32; the output is
+//     fp16, what lb_gemm_int4 takes.
+//   * lowest_t sum(q) is one product more per 8 rows, p_t lowest_t and the sum of p one per 16.
 //   * A tile is 128 rows, one bulk copy; a warp does the scores of 16 of them, the warps exchange maxima, leave p scale in shared memory as operands, and each adds up a
 //     group's 64 features over its part of the tile.
 //   * All tiles of all items are dealt evenly to the CTAs in one line, so that ragged batches balance; an item cut by a border leaves records that kv4_merge joins in order.
@@ -32,25 +34,28 @@ __device__ __forceinline__ float ka_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// exponent of the largest scale, whose fp16 bits are `bits` (16 of them): 2^e <= scale
-__device__ __forceinline__ int ka_exponent(uint32_t bits) {
-    const int e = (__float_as_int(__half2float(__ushort_as_half((unsigned short)bits))) >> 23) - 127;
-    return e < -40 ? -40 : e;
+// fp16 pairs of (x, y) and of what the rounding left
+__device__ __forceinline__ void ka_split(float x, float y, uint32_t& hi, uint32_t& lo) {
+    hi = ka_pack(x, y);
+    const float2 h = ka_pair(hi);
+    lo = ka_pack(x - h.x, y - h.y);
 }
+// 2^(a - e) for scales below 2^(e + 1), whose fp16 bits are at most `bits`; scales below 2^-14 count as that
+__device__ __forceinline__ float ka_against(int a, uint32_t bits) { return ka_pow2(a + 15 - max((int)(bits >> 10), 1)); }
 
 struct ka_item { int r, kv, z, tile, tiles; }; // a place in the line of tiles
 
 template <int D, int MT>
 struct ka {
-    static constexpr int S = D / 64, PARTS = KA_WARPS / S, COLS = 16 * MT, BLK = LB_KV4_BLOCK(D), NS = LB_KV4_STAGES(D, MT);
+    static constexpr int S = D / 64, PARTS = KA_WARPS / S, COLS = LB_KV4_COLS(MT), BLK = LB_KV4_BLOCK(D), NS = LB_KV4_STAGES(D, MT);
     struct alignas(128) smem {
         unsigned char ring[NS][8 * BLK];
         uint4 q[MT][4 * S][32];         // queries as operands of the products: step 4 group + 2 word + u
         uint4 p[S][MT][8][32];          // p scale, likewise: [group][..][16 rows of the tile]
+        uint2 qsum[MT][32];             // sums of a query's groups as the operand that meets (scale, lowest)
         float part[KA_WARPS][COLS][S + 1];
         float max[COLS][KA_WARPS];
-        float factor[COLS], qsum[COLS][S];
-        float m[COLS], l[COLS], low[COLS][S];
+        float factor[COLS], m[COLS], l[COLS], low[COLS][S];
         uint2 scale[KA_WARPS];
         uint64_t full[NS];
         uint32_t pre[LB_KV4_REQS + 1];  // tiles before request r
@@ -58,7 +63,7 @@ struct ka {
         uint32_t warp_sum[KA_WARPS];
     };
 
-    static_assert(sizeof(smem) <= LB_KV4_SMEM(D, MT) && LB_KV4_SMEM(D, MT) * LB_KV4_CTAS(MT) <= 227 * 1024 - 1024 * LB_KV4_CTAS(MT), "shared memory");
+    static_assert(sizeof(smem) <= LB_KV4_SMEM(D, MT) && LB_KV4_SMEM(D, MT) * LB_KV4_CTAS(D, MT) <= 227 * 1024 - 1024 * (LB_KV4_CTAS(D, MT) - 1), "shared memory");
     const lb_kv4_attn_params& p;
     smem& s;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, ft = lane & 3, G;
@@ -171,17 +176,22 @@ struct ka {
             if (lane < D / 8) {
 #pragma unroll
                 for (int u = 0; u < 2; ++u) { // codes n0 n4 | n1 n5 of a word's lower bytes, n2 n6 | n3 n7: the second of a byte comes 2^4 too large
-                    const uint32_t even = ka_pack(x[2 * u] * up, x[2 * u + 4] * up), odd = ka_pack(x[2 * u + 1] * up * 0.0625f, x[2 * u + 5] * up * 0.0625f);
-                    const float2 a = ka_pair(even), b = ka_pair(odd);
-                    sum += (a.x + a.y) + 16.f * (b.x + b.y);
-                    uint32_t* dst = reinterpret_cast<uint32_t*>(&s.q[c >> 4][(lane >> 3) * 4 + 2 * (lane & 1) + u][(c & 7) * 4 + ((lane & 7) >> 1)]) + ((c >> 3) & 1);
-                    dst[0] = even;
-                    dst[2] = odd;
+                    uint4 w;
+                    ka_split(x[2 * u] * up, x[2 * u + 4] * up, w.x, w.y);
+                    ka_split(x[2 * u + 1] * up * 0.0625f, x[2 * u + 5] * up * 0.0625f, w.z, w.w);
+                    const float2 a = ka_pair(w.x), b = ka_pair(w.y), c2 = ka_pair(w.z), d = ka_pair(w.w);
+                    sum += (a.x + a.y) + (b.x + b.y) + 16.f * ((c2.x + c2.y) + (d.x + d.y));
+                    s.q[c >> 3][(lane >> 3) * 4 + 2 * (lane & 1) + u][(c & 7) * 4 + ((lane & 7) >> 1)] = w;
                 }
             }
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane < D / 8 && (lane & 7) == 0) s.qsum[c][lane >> 3] = sum * ka_pow2(-24);
+            sum = __shfl_sync(0xffffffffu, sum, (lane & 3) * 8); // of group lane % 4, at most 2^20
+            if (lane < 4) {
+                uint2 w;
+                ka_split(0.f, lane < S ? sum * 0.015625f : 0.f, w.x, w.y);
+                s.qsum[c >> 3][(c & 7) * 4 + lane] = w;
+            }
             if (lane == 0) {
                 s.factor[c] = ka_pow2(24 - e) * (rsqrtf((float)D) * 1.4426950408889634f); // scores in log2 units
                 s.limit[c] = on ? pos + i : -1;
@@ -189,43 +199,57 @@ struct ka {
         }
     }
 
-    float m[2 * MT], l[2 * MT], low[2 * MT][S]; // of columns 16 mt + g (even) and + 8 (odd): maximum; sums over this thread's rows
-    float acc[MT][8][4];                        // [feature 8 g' + j of the group][columns]
-    int ex[S];                                  // exponent that a group's scales are taken against
+    float m[MT];            // maximum of column 8 mt + g, before its factor
+    float low[MT][4];       // of this warp's rows, columns 8 mt + g in two terms: sums of p lowest of groups 2 ft, 2 ft + 1; ft = 2: the sum of p
+    float acc[MT][8][4];    // [feature 8 (2 ft, 2 ft + 1) + j of the group], likewise in two terms
+    uint2 top;              // fp16 bits of the groups' largest scales so far
 
     __device__ __forceinline__ void begin() {
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.f;
-#pragma unroll
-            for (int q = 0; q < S; ++q) low[i][q] = 0.f;
-        }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt) {
+            m[mt] = -INFINITY;
+            low[mt][0] = low[mt][1] = low[mt][2] = low[mt][3] = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[mt][j][0] = acc[mt][j][1] = acc[mt][j][2] = acc[mt][j][3] = 0.f;
-#pragma unroll
-        for (int q = 0; q < S; ++q) ex[q] = -40;
+        }
+        top = make_uint2(0, 0);
     }
 
     // one tile; false: the wait for it gave up
     __device__ __forceinline__ bool tile(const ka_item& it, int slot, uint32_t parity, bool more, const ka_item& ahead, int ahead_slot) {
-        const bool landed = mbar_wait(&s.full[slot], parity);
         const unsigned char* ring = s.ring[slot];
-        const int nb = blocks(it), row0 = it.tile * LB_KV4_TILE + warp * 16 + 4 * ft, len = s.len[it.r]; // this thread's rows: row0 .. row0 + 3
+        const int len = s.len[it.r], first_new = len - s.n[it.r];
+        const int nb = blocks(it), row0 = it.tile * LB_KV4_TILE + warp * 16 + 4 * ft; // this thread's rows: row0 .. row0 + 3
+        const bool edge = it.tile * LB_KV4_TILE + warp * 16 + 15 > first_new;           // rows that not every column sees, or that are not there
         const unsigned char* blk = ring + warp * BLK;
-        float sc[MT][2][4];
+        float sc[MT][4];
+        uint4 scale[S / 2 < 1 ? 1 : S / 2]; // values' scales of rows row0 .. row0 + 3 as fp16 pairs, two groups each
+        uint2 mx = make_uint2(0, 0);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt) sc[mt][0] = sc[mt][1] = sc[mt][2] = sc[mt][3] = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) sc[mt][i][0] = sc[mt][i][1] = sc[mt][i][2] = sc[mt][i][3] = 0.f;
-        uint32_t top[2] = {0u, 0u};
+        for (int q = 0; q < (S + 1) / 2; ++q) scale[q] = make_uint4(0, 0, 0, 0);
+        const bool landed = mbar_wait(&s.full[slot], parity);
         if (warp < nb && landed) {
+            {   // lowest sum(q)
+                uint32_t b[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) b[i] = *reinterpret_cast<const uint32_t*>(blk + 16 * D + ((ft % S) * 16 + 4 * (g >> 1) + 2 * i + (g & 1)) * 4);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const uint2 a = s.qsum[mt][lane];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float d[4] = {0.f, 0.f, 0.f, 0.f};
+                        ka_mma(d, make_uint4(a.x, a.y, 0u, 0u), b[i], 0u);
+                        sc[mt][2 * i] = (d[0] + d[2]) * 3.814697265625e-06f; // 2^-18: the codes' 2^-24 over the sums' 2^-6
+                        sc[mt][2 * i + 1] = (d[1] + d[3]) * 3.814697265625e-06f;
+                    }
+                }
+            }
 #pragma unroll
             for (int q = 0; q < S; ++q) {
                 const uint4 pr = *reinterpret_cast<const uint4*>(blk + 16 * D + (q * 16 + 4 * ft) * 4);
-                const float2 k0 = ka_pair(pr.x), k1 = ka_pair(pr.y), k2 = ka_pair(pr.z), k3 = ka_pair(pr.w);
                 float a[MT][2][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -245,135 +269,123 @@ struct ka {
                             ka_mma(a[mt][i], qa, v & 0x000f000fu, v & 0x00f000f0u);
                         }
                     }
+                const float k0 = ka_pair(pr.x).x, k1 = ka_pair(pr.y).x, k2 = ka_pair(pr.z).x, k3 = ka_pair(pr.w).x;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
-                    const float q0 = s.qsum[16 * mt + g][q], q1 = s.qsum[16 * mt + 8 + g][q];
-                    sc[mt][0][0] = fmaf(k0.x, a[mt][0][0], fmaf(k0.y, q0, sc[mt][0][0]));
-                    sc[mt][0][1] = fmaf(k1.x, a[mt][0][1], fmaf(k1.y, q0, sc[mt][0][1]));
-                    sc[mt][0][2] = fmaf(k0.x, a[mt][0][2], fmaf(k0.y, q1, sc[mt][0][2]));
-                    sc[mt][0][3] = fmaf(k1.x, a[mt][0][3], fmaf(k1.y, q1, sc[mt][0][3]));
-                    sc[mt][1][0] = fmaf(k2.x, a[mt][1][0], fmaf(k2.y, q0, sc[mt][1][0]));
-                    sc[mt][1][1] = fmaf(k3.x, a[mt][1][1], fmaf(k3.y, q0, sc[mt][1][1]));
-                    sc[mt][1][2] = fmaf(k2.x, a[mt][1][2], fmaf(k2.y, q1, sc[mt][1][2]));
-                    sc[mt][1][3] = fmaf(k3.x, a[mt][1][3], fmaf(k3.y, q1, sc[mt][1][3]));
+                    sc[mt][0] = fmaf(k0, a[mt][0][0] + a[mt][0][2], sc[mt][0]);
+                    sc[mt][1] = fmaf(k1, a[mt][0][1] + a[mt][0][3], sc[mt][1]);
+                    sc[mt][2] = fmaf(k2, a[mt][1][0] + a[mt][1][2], sc[mt][2]);
+                    sc[mt][3] = fmaf(k3, a[mt][1][1] + a[mt][1][3], sc[mt][3]);
                 }
-                const uint4 vr = *reinterpret_cast<const uint4*>(blk + 17 * D + (q * 16 + 4 * ft) * 4);
-                uint32_t mx = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t b = (i == 0 ? vr.x : i == 1 ? vr.y : i == 2 ? vr.z : vr.w) & 0xffffu; // scales are not negative; a NaN's group has no say here
-                    if (row0 + i < len && b < 0x7c00u) mx = max(mx, b);
-                }
-                top[q >> 1] |= mx << (16 * (q & 1));
+                uint4 vr = *reinterpret_cast<const uint4*>(blk + 17 * D + (q * 16 + 4 * ft) * 4);
+                if (edge) vr = there(vr, row0, len);
+                uint32_t& s01 = q & 1 ? scale[q >> 1].z : scale[q >> 1].x;
+                uint32_t& s23 = q & 1 ? scale[q >> 1].w : scale[q >> 1].y;
+                s01 = __byte_perm(vr.x, vr.y, 0x5410);
+                s23 = __byte_perm(vr.z, vr.w, 0x5410);
             }
-        }
-        float mx[2 * MT];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) { // columns 16 mt + g + 8 e: the scores of rows row0 .. row0 + 3
-                const int c = 16 * mt + 8 * e + g, lim = warp < nb ? s.limit[c] : -1;
-                const float f = s.factor[c];
-                float v = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float& x = sc[mt][i >> 1][2 * e + (i & 1)];
-                    x = row0 + i <= lim ? x * f : -INFINITY;
-                    v = fmaxf(v, x);
+            // the largest scale of each group over these rows; scales are not negative
+            auto most = [&](uint4 v) {
+                if (edge) { // a NaN has no say: columns before its row are not to notice it
+                    v.x &= __vcmpltu2(v.x, 0x7c007c00u); v.y &= __vcmpltu2(v.y, 0x7c007c00u);
+                    v.z &= __vcmpltu2(v.z, 0x7c007c00u); v.w &= __vcmpltu2(v.w, 0x7c007c00u);
                 }
-                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-                v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-                mx[2 * mt + e] = v;
-                if (ft == 0) s.max[c][warp] = v;
-            }
+                const uint32_t a = __vmaxu2(v.x, v.y), b = __vmaxu2(v.z, v.w);
+                return __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+            };
+            mx.x = most(scale[0]);
+            if (S > 2) mx.y = most(scale[S / 2 < 1 ? 0 : S / 2 - 1]);
+            if (edge) {
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            top[0] = __vmaxu2(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
-            if (S > 2) top[1] = __vmaxu2(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
-        }
-        if (lane == 0) s.scale[warp] = make_uint2(top[0], top[1]);
-        if (__syncthreads_or(!landed)) return false;
-        // everybody is done with the tile before: its slot is free
-        if (t == 0 && more) fetch(ahead, ahead_slot);
-        float corr[2 * MT];
+                for (int mt = 0; mt < MT; ++mt) {
+                    const int lim = s.limit[8 * mt + g];
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-            const float* row = s.max[16 * (i >> 1) + 8 * (i & 1) + g];
-            const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
-            const float now = fmaxf(fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))), m[i]);
-            mx[i] = now == -INFINITY ? 0.f : now; // a column that has seen nothing yet
-            corr[i] = ka_exp2(m[i] - mx[i]);
-            m[i] = now;
-            l[i] *= corr[i];
-        }
-        uint2 tp = s.scale[0];
-#pragma unroll
-        for (int w = 1; w < KA_WARPS; ++w) {
-            const uint2 v = s.scale[w];
-            tp.x = __vmaxu2(tp.x, v.x);
-            if (S > 2) tp.y = __vmaxu2(tp.y, v.y);
-        }
-        const int group = warp % S, part = warp / S;
-        float shrink = 1.f; // of this warp's group: its scales are taken against a larger one from here on
-#pragma unroll
-        for (int q = 0; q < S; ++q) {
-            const int e = max(ex[q], ka_exponent(((q & 2 ? tp.y : tp.x) >> (16 * (q & 1))) & 0xffffu));
-            if (q == group) shrink = ka_pow2(ex[q] - e);
-            ex[q] = e;
-        }
-        // probabilities
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float& x = sc[mt][i >> 1][2 * e + (i & 1)];
-                    x = ka_exp2(x - mx[2 * mt + e]);
-                    l[2 * mt + e] += x;
+                    for (int i = 0; i < 4; ++i)
+                        if (row0 + i > lim) sc[mt][i] = -INFINITY;
                 }
-#pragma unroll
-        for (int q = 0; q < S; ++q) {
-            uint4 vr = make_uint4(0, 0, 0, 0);
-            if (warp < nb) vr = *reinterpret_cast<const uint4*>(blk + 17 * D + (q * 16 + 4 * ft) * 4);
-            if (row0 + 3 >= len) { // rows behind the last one may hold anything
-                if (row0 >= len) vr.x = 0;
-                if (row0 + 1 >= len) vr.y = 0;
-                if (row0 + 2 >= len) vr.z = 0;
-                vr.w = 0;
-            }
-            if (row0 + 3 > len - s.n[it.r]) { // new rows, which not every column sees: a NaN's group reaches those that do, and no other by way of 0 times NaN
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t& v = i == 0 ? vr.x : i == 1 ? vr.y : i == 2 ? vr.z : vr.w;
-                    if ((v & 0x7fffu) < 0x7c00u) continue;
-                    v = 0;
-#pragma unroll
-                    for (int c = 0; c < 2 * MT; ++c)
-                        if (row0 + i <= s.limit[16 * (c >> 1) + 8 * (c & 1) + g]) low[c][q] = NAN;
-                }
-            }
-            const float2 v0 = ka_pair(vr.x), v1 = ka_pair(vr.y), v2 = ka_pair(vr.z), v3 = ka_pair(vr.w);
-            const float up = ka_pow2(13 - ex[q]);
-            const float s0 = v0.x * up, s1 = v1.x * up, s2 = v2.x * up, s3 = v3.x * up;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float& lo = low[2 * mt + e][q];
-                    lo = fmaf(sc[mt][0][2 * e], v0.y, fmaf(sc[mt][0][2 * e + 1], v1.y, fmaf(sc[mt][1][2 * e], v2.y, fmaf(sc[mt][1][2 * e + 1], v3.y, lo * corr[2 * mt + e]))));
-                }
-                if (warp < nb)
-                    s.p[q][mt][warp][lane] = make_uint4(ka_pack(sc[mt][0][0] * s0, sc[mt][0][1] * s1), ka_pack(sc[mt][0][2] * s0, sc[mt][0][3] * s1),
-                                                        ka_pack(sc[mt][1][0] * s2, sc[mt][1][1] * s3), ka_pack(sc[mt][1][2] * s2, sc[mt][1][3] * s3));
             }
         }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-            const float c0 = corr[2 * mt] * shrink, c1 = corr[2 * mt + 1] * shrink;
-            if (__any_sync(0xffffffffu, c0 != 1.f || c1 != 1.f)) {
+            float v = fmaxf(fmaxf(sc[mt][0], sc[mt][1]), fmaxf(sc[mt][2], sc[mt][3]));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+            if (ft == 0) s.max[8 * mt + g][warp] = v;
+        }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { acc[mt][j][0] *= c0; acc[mt][j][1] *= c0; acc[mt][j][2] *= c1; acc[mt][j][3] *= c1; }
+        for (int o = 1; o < 4; o <<= 1) {
+            mx.x = __vmaxu2(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o));
+            if (S > 2) mx.y = __vmaxu2(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o));
+        }
+        if (lane == 0) s.scale[warp] = mx;
+        if (__syncthreads_or(!landed)) return false;
+        // everybody is done with the tile before: its slot is free
+        if (t == 0 && more) fetch(ahead, ahead_slot);
+        const uint2 old = top;
+#pragma unroll
+        for (int w = 0; w < KA_WARPS; ++w) {
+            const uint2 v = s.scale[w];
+            top.x = __vmaxu2(top.x, v.x);
+            if (S > 2) top.y = __vmaxu2(top.y, v.y);
+        }
+        const int group = warp % S, part = warp / S;
+        auto bits = [](const uint2& v, int q) { return ((q & 2 ? v.y : v.x) >> (16 * (q & 1))) & 0xffffu; };
+        const float shrink = ka_against(0, bits(top, group)) * ka_pow2(max((int)(bits(old, group) >> 10), 1) - 15); // this warp's group is taken against a larger scale from here on
+        float corr[MT];
+        uint2 hi[MT], lo[MT]; // probabilities, times 2^14
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const float* row = s.max[8 * mt + g];
+            const float4 a = *reinterpret_cast<const float4*>(row), b = *reinterpret_cast<const float4*>(row + 4);
+            const float f = s.factor[8 * mt + g], now = fmaxf(fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))), m[mt]);
+            const float less = now == -INFINITY ? 0.f : -now * f; // a column that has seen nothing yet
+            corr[mt] = ka_exp2(fmaf(m[mt], f, less));
+            m[mt] = now;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[mt][i] = ka_exp2(fmaf(sc[mt][i], f, less + 14.f));
+            ka_split(sc[mt][0], sc[mt][1], hi[mt].x, lo[mt].x);
+            ka_split(sc[mt][2], sc[mt][3], hi[mt].y, lo[mt].y);
+        }
+        if (__any_sync(0xffffffffu, differs(corr, shrink))) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float c = corr[mt] * shrink;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) low[mt][i] *= corr[mt];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { acc[mt][j][0] *= c; acc[mt][j][1] *= c; acc[mt][j][2] *= c; acc[mt][j][3] *= c; }
+            }
+        }
+        if (warp < nb) {
+            uint4 vr = *reinterpret_cast<const uint4*>(blk + 17 * D + ((g % S) * 16 + 4 * ft) * 4);
+            if (edge) { // NaNs of rows that a column does not see must not reach it as 0 times NaN; where it does, p scale is NaN
+                vr = there(vr, row0, len);
+                vr.x = lowest_or_0(vr.x); vr.y = lowest_or_0(vr.y); vr.z = lowest_or_0(vr.z); vr.w = lowest_or_0(vr.w);
+            }
+            const uint32_t b0 = g == 4 ? 0x3c003c00u : __byte_perm(vr.x, vr.y, 0x7632), b1 = g == 4 ? 0x3c003c00u : __byte_perm(vr.z, vr.w, 0x7632);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) ka_mma(low[mt], make_uint4(hi[mt].x, lo[mt].x, hi[mt].y, lo[mt].y), b0, b1);
+#pragma unroll
+            for (int q = 0; q < S; ++q) {
+                const float up = ka_against(-1, bits(top, q));
+                const float2 s01 = ka_pair(q & 1 ? scale[q >> 1].z : scale[q >> 1].x), s23 = ka_pair(q & 1 ? scale[q >> 1].w : scale[q >> 1].y);
+                const float v[4] = {s01.x * up, s01.y * up, s23.x * up, s23.y * up};
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = sc[mt][i] * v[i];
+                    if (edge) {
+                        const int lim = s.limit[8 * mt + g];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (row0 + i > lim) w[i] = 0.f;
+                    }
+                    uint4 o;
+                    ka_split(w[0], w[1], o.x, o.y);
+                    ka_split(w[2], w[3], o.z, o.w);
+                    s.p[q][mt][warp][lane] = o;
+                }
             }
         }
         __syncthreads();
@@ -398,32 +410,32 @@ struct ka {
         }
         return true;
     }
+    static __device__ __forceinline__ bool differs(const float (&corr)[MT], float shrink) {
+        bool d = shrink != 1.f;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) d |= corr[mt] != 1.f;
+        return d;
+    }
+    // (scale, lowest) of four rows, of those that are there
+    static __device__ __forceinline__ uint4 there(uint4 v, int row0, int len) {
+        return make_uint4(row0 < len ? v.x : 0u, row0 + 1 < len ? v.y : 0u, row0 + 2 < len ? v.z : 0u, row0 + 3 < len ? v.w : 0u);
+    }
+    static __device__ __forceinline__ uint32_t lowest_or_0(uint32_t pair) { return (pair & 0x7fff0000u) < 0x7c000000u ? pair : 0u; }
 
     // The item's columns, whole or this CTA's share of them: out, or a record.  `first`: the item's first tile was this CTA's, `last`: its last
     __device__ __forceinline__ void finish(const ka_item& it, bool first, bool last) {
         float* sum = reinterpret_cast<float*>(&s.p[0][0][0][0]); // [COLS][D]
         const int group = warp % S, part = warp / S, cols = min(COLS, s.n[it.r] * G - it.z * COLS);
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {
-            const int c = 16 * (i >> 1) + 8 * (i & 1) + g;
-            float v = l[i];
-            v += __shfl_xor_sync(0xffffffffu, v, 1);
-            v += __shfl_xor_sync(0xffffffffu, v, 2);
-            if (ft == 0) s.part[warp][c][S] = v;
-#pragma unroll
-            for (int q = 0; q < S; ++q) {
-                v = low[i][q];
-                v += __shfl_xor_sync(0xffffffffu, v, 1);
-                v += __shfl_xor_sync(0xffffffffu, v, 2);
-                if (ft == 0) s.part[warp][c][q] = v;
-            }
-            if (ft == 0 && warp == 0) s.m[c] = m[i];
+        for (int mt = 0; mt < MT; ++mt) {
+            const int c = 8 * mt + g;
+            if (2 * ft < S) s.part[warp][c][2 * ft] = low[mt][0] + low[mt][2];
+            if (2 * ft + 1 < S) s.part[warp][c][2 * ft + 1] = low[mt][1] + low[mt][3];
+            if (ft == 2) s.part[warp][c][S] = low[mt][0] + low[mt][2];
+            if (ft == 0 && warp == 0) s.m[c] = m[mt] == -INFINITY ? m[mt] : m[mt] * s.factor[c];
         }
-        int e = 0;
-#pragma unroll
-        for (int q = 0; q < S; ++q)
-            if (q == group) e = ex[q];
-        const float even = ka_pow2(e + 11), odd = ka_pow2(e + 7); // 2^24 (2^20) over 2^(13 - e)
+        const int e = max((int)(((group & 2 ? top.y : top.x) >> (16 * (group & 1)) & 0xffffu) >> 10), 1) - 15;
+        const float even = ka_pow2(e + 25), odd = ka_pow2(e + 21); // 2^24 (2^20) over 2^(-1 - e)
         for (int turn = 0; turn < PARTS; ++turn) { // the parts of a tile one after the other
             __syncthreads();
             if (part == turn)
@@ -432,9 +444,9 @@ struct ka {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float& x = sum[(16 * mt + g + (i & 2 ? 8 : 0)) * D + group * 64 + 8 * (2 * ft + (i & 1)) + j];
-                            const float y = acc[mt][j][i] * (j & 1 ? odd : even);
+                        for (int i = 0; i < 2; ++i) {
+                            float& x = sum[(8 * mt + g) * D + group * 64 + 8 * (2 * ft + i) + j];
+                            const float y = (acc[mt][j][i] + acc[mt][j][2 + i]) * (j & 1 ? odd : even);
                             x = turn ? x + y : y;
                         }
         }
@@ -545,7 +557,7 @@ struct ka {
 };
 
 #define KA_KERNEL(D, MT)                                                                                                                             \
-    extern "C" __global__ void __launch_bounds__(KA_THREADS, LB_KV4_CTAS(MT)) kv4_attn_##D##_##MT(const __grid_constant__ lb_kv4_attn_params p) {   \
+    extern "C" __global__ void __launch_bounds__(KA_THREADS, LB_KV4_CTAS(D, MT)) kv4_attn_##D##_##MT(const __grid_constant__ lb_kv4_attn_params p) {   \
         extern __shared__ __align__(128) unsigned char ka_sm[];                                                                                     \
         ka<D, MT> k(p, *reinterpret_cast<ka<D, MT>::smem*>(ka_sm));                                                                                  \
         k.body();                                                                                                                                    \
@@ -556,30 +568,64 @@ KA_KERNEL(256, 1)
 KA_KERNEL(64, 2)
 KA_KERNEL(128, 2)
 KA_KERNEL(256, 2)
+KA_KERNEL(64, 4)
+KA_KERNEL(128, 4)
+KA_KERNEL(256, 4)
 
-// Joins the records of the items that were cut: CTA (b, y) those of the item whose first cut is the border before CTA b, columns y, y + gridDim.y, ...
-// Records are added in the order of the rows, so results are the same from run to run.
+// Joins the records of the items that were cut.  Every CTA lists the joins; (join, column) pairs are dealt to the CTAs.  Records are added in the order of the rows, in runs
+// of neighbours side by side, so results are the same from run to run.
 #define KM_THREADS 1024
+#define KM_JOINS 512 /* CTAs of the attention kernel at most */
 template <int D>
-__device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int slots) {
+__device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int ctas, int slots) {
     constexpr int SUB = KM_THREADS / D; // runs of records side by side
     __shared__ float red[3][KM_THREADS];
+    __shared__ int s_join[KM_JOINS], s_before[KM_JOINS + 1], s_warp[KM_JOINS / 32][2];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     pdl_wait();
-    const lb_kv4_join j = p.joins[blockIdx.x];
-    if (j.first < 0) return;
-    const int f = threadIdx.x % D, sub = threadIdx.x / D, G = p.HQ / p.b.HKV, per = (j.last - j.first + SUB) / SUB; // records of a run
-    for (int c = blockIdx.y; c < j.cols; c += gridDim.y) {
+    int cols = 0;
+    if (t < ctas && p.joins[t].first >= 0) cols = p.joins[t].cols;
+    const uint32_t on = __ballot_sync(0xffffffffu, cols > 0);
+    int sum = cols;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 31 && warp < KM_JOINS / 32) {
+        s_warp[warp][0] = __popc(on);
+        s_warp[warp][1] = sum;
+    }
+    __syncthreads();
+    int joins = 0, pairs = 0, at = __popc(on & ((1u << lane) - 1u)), before = sum - cols;
+#pragma unroll
+    for (int w = 0; w < KM_JOINS / 32; ++w) {
+        if (w == warp) { at += joins; before += pairs; }
+        joins += s_warp[w][0];
+        pairs += s_warp[w][1];
+    }
+    if (cols > 0) {
+        s_join[at] = t;
+        s_before[at] = before;
+    }
+    __syncthreads();
+    const int f = t % D, sub = t / D, G = p.HQ / p.b.HKV;
+    int k = 0;
+    for (int pair = blockIdx.x; pair < pairs; pair += gridDim.x) {
+        while (k + 1 < joins && s_before[k + 1] <= pair) ++k;
+        const lb_kv4_join j = p.joins[s_join[k]];
+        const int c = pair - s_before[k], per = (j.last - j.first + SUB) / SUB; // records of a run
         float M = -INFINITY, L = 0.f, A = 0.f;
         const int b0 = j.first + sub * per, b1 = min(j.last + 1, b0 + per);
         for (int b = b0; b < b1; b += 8) {
             float mv[8], lv[8], av[8], mx = M;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bool on = b + i < b1;
-                const float* rec = p.records + (((size_t)(on ? b + i : b) * 2 + (b + i == j.first ? 1 : 0)) * slots + c) * LB_KV4_REC(D);
-                mv[i] = on ? __ldcg(rec + D) : -INFINITY;
-                lv[i] = on ? __ldcg(rec + D + 1) : 0.f;
-                av[i] = on ? __ldcg(rec + f) : 0.f;
+                const bool there = b + i < b1;
+                const float* rec = p.records + (((size_t)(there ? b + i : b) * 2 + (b + i == j.first ? 1 : 0)) * slots + c) * LB_KV4_REC(D);
+                mv[i] = there ? __ldcg(rec + D) : -INFINITY;
+                lv[i] = there ? __ldcg(rec + D + 1) : 0.f;
+                av[i] = there ? __ldcg(rec + f) : 0.f;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) mx = fmaxf(mx, mv[i]);
@@ -594,9 +640,9 @@ __device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int 
             }
             M = mx;
         }
-        red[0][threadIdx.x] = M;
-        red[1][threadIdx.x] = L;
-        red[2][threadIdx.x] = A;
+        red[0][t] = M;
+        red[1][t] = L;
+        red[2][t] = A;
         __syncthreads();
         if (sub == 0) {
             float mx = M;
@@ -619,6 +665,6 @@ __device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int 
         __syncthreads();
     }
 }
-extern "C" __global__ void __launch_bounds__(KM_THREADS) kv4_merge_64(const __grid_constant__ lb_kv4_attn_params p, int slots) { kv4_merge_body<64>(p, slots); }
-extern "C" __global__ void __launch_bounds__(KM_THREADS) kv4_merge_128(const __grid_constant__ lb_kv4_attn_params p, int slots) { kv4_merge_body<128>(p, slots); }
-extern "C" __global__ void __launch_bounds__(KM_THREADS) kv4_merge_256(const __grid_constant__ lb_kv4_attn_params p, int slots) { kv4_merge_body<256>(p, slots); }
+extern "C" __global__ void __launch_bounds__(KM_THREADS) kv4_merge_64(const __grid_constant__ lb_kv4_attn_params p, int ctas, int slots) { kv4_merge_body<64>(p, ctas, slots); }
+extern "C" __global__ void __launch_bounds__(KM_THREADS) kv4_merge_128(const __grid_constant__ lb_kv4_attn_params p, int ctas, int slots) { kv4_merge_body<128>(p, ctas, slots); }
+extern "C" __global__ void __launch_bounds__(KM_THREADS) kv4_merge_256(const __grid_constant__ lb_kv4_attn_params p, int ctas, int slots) { kv4_merge_body<256>(p, ctas, slots); }

@@ -599,11 +599,10 @@ typedef struct {
     int32_t pad_;
     double freq[128];
 } lb_kv4_attn_params;
-/* rings of the attention kernel: two CTAs per SM of 16 columns, or one of 32 */
-#define LB_KV4_STAGES(D, MT) ((D) == 256 ? ((MT) == 1 ? 2 : 4) : (D) == 128 ? ((MT) == 1 ? 4 : 6) : 6)
-#define LB_KV4_CTAS(MT) ((MT) == 1 ? 2 : 1) /* per SM */
-#define LB_KV4_COLS(MT) (16 * (MT))
-/* ring, queries, probabilities, the rest */
-#define LB_KV4_SMEM(D, MT) (LB_KV4_STAGES(D, MT) * 8 * LB_KV4_BLOCK(D) + (MT) * (D) * 32 + (MT) * (D) * 64 + 6 * 1024 + (MT) * 4 * 1024)
+/* Columns taken at a time, CTAs per SM and ring stages of the attention kernel's variants.  A CTA uses its shared memory for the ring, queries, probabilities, the rest */
+#define LB_KV4_COLS(MT) (8 * (MT))
+#define LB_KV4_CTAS(D, MT) ((MT) == 1 ? 2 : 1)
+#define LB_KV4_STAGES(D, MT) ((D) == 256 ? ((MT) == 4 ? 3 : (MT) == 2 ? 4 : 2) : (MT) == 1 && (D) == 128 ? 4 : 6)
+#define LB_KV4_SMEM(D, MT) (LB_KV4_STAGES(D, MT) * 8 * LB_KV4_BLOCK(D) + (MT) * (D) * 32 + (MT) * (D) * 64 + 6 * 1024 + (MT) * 2 * 1024)
 
 #endif
