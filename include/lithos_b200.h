@@ -312,6 +312,20 @@ int lb_kv4_read(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batc
  * kv_heads.  max_new: the most tokens a request of the batch has, 1 .. LB_KV4_MAX_NEW.  out fp16 [rows, n_heads, dim], what lb_gemm_int4 takes. */
 int lb_kv4_attention(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t q, uint64_t gate, int64_t row_stride, int64_t head_stride, int type,
                      uint64_t q_norm_w, uint64_t out_f16, int n_heads, int max_new, int rot_dims, float rope_theta, float eps);
+/* Drafted tokens against the target's probabilities, for speculative decoding (with lb_model_checkpoint / lb_model_rollback for a model's recurrent state, or over the
+ * cache above, where rows behind the accepted ones are simply written again).  Rows starts[r] .. starts[r+1]-1 of logits [rows, vocab] fp32 are the target's after request r's
+ * tokens so far and after each of its drafts: one row more than drafts.  drafts i32 [rows]: row j's draft, the token drafted from where row j stands (the entry of a request's
+ * last row is not read as one).  p = softmax(logits / temperature) over the top_k (1..64) largest logits, ties by smaller index, as lb_sample_topk, or over the whole
+ * vocabulary (top_k = 0); temperature <= 0: greedy, p = 1 at the arg-max.  q: the draft's probabilities, draft_probs fp32 [rows, vocab] (rows of last rows are not read), or 1 at the
+ * draft where draft_probs = 0 (drafts that were not drawn).  Logits of -infinity or NaN have probability 0.
+ *   Row by row a draft x stands while  u_accept[row] * q(x) < p(x)  (greedy: while it is the arg-max).  The first row that does not stand, or the last one, gives the token: the
+ * first one, by index (top_k: by rank), at which the running sum of weights exceeds u_pick[r] times the whole, weights max(p - q, 0), at the last row p (and where the former are all
+ * 0).  All of that is computed in 64 bits.
+ * tokens i32 [rows]: the drafts that stand, the token, then -1; accepted i32 [n_reqs]: how many stand, -1 for a request without rows; p_out fp32 [rows] (0: not wanted):
+ * p of every draft, 0 in last rows.  Rows behind the last request's are left as they were; a request that names rows that are not there gets -1, status word 0x1006. */
+enum { LB_VERIFY_MAX_REQS = 256, LB_VERIFY_MAX_ROWS = 8192 };
+int lb_verify_drafts(lb_ctx* ctx, uint64_t logits_f32, int vocab, uint64_t starts, int n_reqs, int rows, uint64_t drafts, uint64_t draft_probs, uint64_t u_accept, uint64_t u_pick,
+                     uint64_t tokens, uint64_t accepted, double temperature, int top_k, uint64_t p_out);
 
 /* ---- small kernels ---------------------------------------------------------------------
  * rmsnorm: replaces launch_norm (src/launcher.s:1101-1219, inference/reduce.ls:21-147);

@@ -132,6 +132,7 @@ def lib() -> C.CDLL:
     sig("lb_kv4_append", i32, vp, KC, KB, u64, u64, i64, i32, u64, i32, f32, f32)
     sig("lb_kv4_read", i32, vp, KC, KB, u64, u64, i32)
     sig("lb_kv4_attention", i32, vp, KC, KB, u64, u64, i64, i64, i32, u64, u64, i32, i32, i32, f32, f32)
+    sig("lb_verify_drafts", i32, vp, u64, i32, u64, i32, i32, u64, u64, u64, u64, u64, u64, C.c_double, i32, u64)
     _lib = L
     return L
 
@@ -446,6 +447,11 @@ class Context:
     def sample_topk(self, x, n, temperature, top_k, seed, counter, out_idx, probs_out=None, idx_out=None):
         self._check(lib().lb_sample_topk(self.h, x.ptr, n, temperature, top_k, seed, counter, out_idx.ptr,
                                          probs_out.ptr if probs_out else 0, idx_out.ptr if idx_out else 0))
+
+    def verify_drafts(self, logits, vocab, starts, n_reqs, rows, drafts, draft_probs, u_accept, u_pick, tokens, accepted, temperature=1.0, top_k=0, p_out=None):
+        """drafted tokens held against the target's probabilities: how many of each request stand, and the token that follows them"""
+        self._check(lib().lb_verify_drafts(self.h, logits.ptr, vocab, starts.ptr, n_reqs, rows, drafts.ptr, draft_probs.ptr if draft_probs else 0, u_accept.ptr, u_pick.ptr,
+                                           tokens.ptr, accepted.ptr, temperature, top_k, p_out.ptr if p_out else 0))
 
     def embed(self, table, token, out, D):
         self._check(lib().lb_embed(self.h, table.ptr, token.ptr, out.ptr, D))

@@ -129,7 +129,7 @@ static int load_cubin(lb_ctx* c, const char* dir, const char* file) {
 
 static const char* const k_cubins[] = {"gemv.cubin", "chain.cubin", "batched.cubin", "batched_tc.cubin", "batched_ring.cubin", "deltanet.cubin", "attention.cubin", "attention_mma.cubin", "small.cubin", "comm.cubin", "prefill.cubin",
                                        "rows_gemv.cubin", "dense_gemm.cubin", "window_attention.cubin", "decay_attention.cubin",
-                                       "latent_attention.cubin", "ssm.cubin", "ssm_tc.cubin", "kv4_cache.cubin", "kv4_attention.cubin"};
+                                       "latent_attention.cubin", "ssm.cubin", "ssm_tc.cubin", "kv4_cache.cubin", "kv4_attention.cubin", "verify.cubin"};
 
 LB_API int lb_init(int device, const char* kernel_dir, lb_ctx** out) { return lb_init_images(device, kernel_dir, NULL, out); }
 
@@ -214,6 +214,7 @@ LB_API int lb_init_images(int device, const char* kernel_dir, const char* images
         LB_CU(c, lb_drv.MemAlloc(&c->kv4_records, recs + 2 * (size_t)c->sm_count * sizeof(lb_kv4_join)));
         c->kv4_joins = c->kv4_records + recs;
     }
+    if (c->fn[LBK_vd_rows]) LB_CU(c, lb_drv.MemAlloc(&c->vd_stat, (size_t)LB_VD_ROWS * (sizeof(lb_vd_row) + LB_VD_TOPK * 8)));
     LB_CU(c, lb_drv.MemAlloc(&c->chain_mail, (size_t)LB_CHAIN_MAX_OPS * LB_CHAIN_MAIL_WORDS * 8));
     LB_CU(c, lb_drv.MemsetD8Async(c->chain_mail, 0, (size_t)LB_CHAIN_MAX_OPS * LB_CHAIN_MAIL_WORDS * 8, c->stream));
     c->chain_mailbox = 1;
@@ -237,6 +238,7 @@ LB_API void lb_destroy(lb_ctx* c) {
         if (c->gemv_partial) lb_drv.MemFree(c->gemv_partial);
         if (c->gemv_counters) lb_drv.MemFree(c->gemv_counters);
         if (c->attn_scratch) lb_drv.MemFree(c->attn_scratch);
+        if (c->vd_stat) lb_drv.MemFree(c->vd_stat);
         if (c->kv4_records) lb_drv.MemFree(c->kv4_records);
         if (c->dev_status) lb_drv.MemFree(c->dev_status);
         if (c->chain_mail) lb_drv.MemFree(c->chain_mail);

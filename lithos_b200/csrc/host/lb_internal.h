@@ -198,6 +198,10 @@ int lb_driver_load(char* err, size_t errlen); /* LB_OK or LB_ERR_NO_DRIVER */
     X(ssm_tc)                         \
     X(ssm_tc_local)                   \
     X(ssm_finish)                     \
+    X(vd_rows)                        \
+    X(vd_rows_topk)                   \
+    X(vd_pick_short)                  \
+    X(vd_pick)                        \
     X(kv4_append_64)                  \
     X(kv4_append_128)                 \
     X(kv4_append_256)                 \
@@ -248,6 +252,7 @@ struct lb_ctx {
     size_t attn_scratch_bytes;
     CUdeviceptr kv4_records;   /* partial results of the batch attention, then its joins; made with the context when its kernels are loaded */
     CUdeviceptr kv4_joins;
+    CUdeviceptr vd_stat;       /* rows of lb_verify_drafts, then their lists of candidates */
     CUdeviceptr dev_status; /* u32 words written by bounded device-side waits */
     CUdeviceptr flush_buf;  /* L2 flush target */
     size_t flush_bytes;

@@ -99,7 +99,7 @@ struct ka {
         return total;
     }
     __device__ __forceinline__ ka_item place(uint32_t x) const {
-        int lo = 0, hi = LB_KV4_REQS - 1; // the last request with pre <= x that has tiles
+        int lo = 0, hi = p.b.n_reqs - 1; // the last request with pre <= x that has tiles
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (s.pre[mid] <= x) lo = mid;
@@ -121,8 +121,8 @@ struct ka {
         it.z = 0;
         if (++it.kv < p.b.HKV) return;
         it.kv = 0;
-        do ++it.r; while (it.r < LB_KV4_REQS && s.n[it.r] <= 0);
-        it.tiles = it.r < LB_KV4_REQS ? (s.len[it.r] + LB_KV4_TILE - 1) / LB_KV4_TILE : 0;
+        do ++it.r; while (it.r < p.b.n_reqs && s.n[it.r] <= 0);
+        it.tiles = it.r < p.b.n_reqs ? (s.len[it.r] + LB_KV4_TILE - 1) / LB_KV4_TILE : 0;
     }
     __device__ __forceinline__ int blocks(const ka_item& it) const { return min(8, (s.len[it.r] - it.tile * LB_KV4_TILE + 15) >> 4); }
     __device__ __forceinline__ void fetch(const ka_item& it, int slot) const {
@@ -501,8 +501,8 @@ struct ka {
         uint32_t fetched = x0;
         if (t == 0) {
             for (; fetched < x1 && fetched < x0 + NS - 1; ++fetched) {
+                if (fetched > x0) next(ahead);
                 fetch(ahead, (int)(fetched - x0));
-                next(ahead);
             }
             // does an item begin in the CTA before and go on here?
             lb_kv4_join j;
@@ -529,6 +529,7 @@ struct ka {
                 __syncthreads();
             }
             const bool more = fetched < x1;
+            if (t == 0 && more) next(ahead);
             const int ahead_slot = slot ? slot - 1 : NS - 1;
             if (!tile(it, slot, parity, more, ahead, ahead_slot)) { // a copy never landed: say so, let the others land, leave
                 if (t == 0) {
@@ -541,16 +542,13 @@ struct ka {
                 __syncthreads();
                 return;
             }
-            if (t == 0 && more) {
-                ++fetched;
-                next(ahead);
-            }
+            if (t == 0 && more) ++fetched;
             if (++slot == NS) { slot = 0; parity ^= 1u; }
             if (it.tile == it.tiles - 1 || x == x1 - 1) {
                 __syncthreads();
                 finish(it, first, it.tile == it.tiles - 1);
             }
-            next(it);
+            if (x + 1 < x1) next(it);
         }
         pdl_launch_dependents();
     }

@@ -605,4 +605,34 @@ typedef struct {
 #define LB_KV4_STAGES(D, MT) ((D) == 256 ? ((MT) == 4 ? 3 : (MT) == 2 ? 4 : 2) : (MT) == 1 && (D) == 128 ? 4 : 6)
 #define LB_KV4_SMEM(D, MT) (LB_KV4_STAGES(D, MT) * 8 * LB_KV4_BLOCK(D) + (MT) * (D) * 32 + (MT) * (D) * 64 + 6 * 1024 + (MT) * 2 * 1024)
 
+/* ---- drafted tokens against the target's probabilities (verify.cu) -------------------------------------------- */
+#define LB_VD_REQS 256
+#define LB_VD_ROWS 8192
+#define LB_VD_TOPK 64
+#define LB_VD_CLUSTER 8 /* CTAs of a row or a request at most */
+typedef struct {
+    double z;          /* sum of exp((l - max) / temperature) over the tokens that count */
+    float max;
+    int32_t best;      /* first index of the maximum */
+    int32_t stands;    /* the row's draft is accepted */
+    int32_t n;         /* candidates in the row's list (top-k) */
+} lb_vd_row;
+typedef struct {
+    const float* logits;    /* [rows, V] */
+    const int32_t* starts;  /* [n_reqs + 1] */
+    const int32_t* drafts;  /* [rows] */
+    const float* probs;     /* [rows, V] the draft's probabilities, or NULL: certain drafts */
+    const float* u_accept;  /* [rows] */
+    const float* u_pick;    /* [n_reqs] */
+    int32_t* tokens;        /* [rows] */
+    int32_t* accepted;      /* [n_reqs] */
+    float* p_out;           /* [rows] or NULL */
+    lb_vd_row* stat;        /* [rows] */
+    float* list_val;        /* [rows][LB_VD_TOPK] */
+    int32_t* list_idx;
+    uint32_t* status;
+    double temperature;     /* <= 0: greedy */
+    int32_t V, n_reqs, rows, top_k; /* top_k 0: the whole vocabulary */
+} lb_vd_params;
+
 #endif
