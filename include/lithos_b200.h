@@ -316,7 +316,7 @@ int lb_kv4_attention(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch*
  * cache above, where rows behind the accepted ones are simply written again).  Rows starts[r] .. starts[r+1]-1 of logits [rows, vocab] fp32 are the target's after request r's
  * tokens so far and after each of its drafts: one row more than drafts.  drafts i32 [rows]: row j's draft, the token drafted from where row j stands (the entry of a request's
  * last row is not read as one).  p = softmax(logits / temperature) over the top_k (1..64) largest logits, ties by smaller index, as lb_sample_topk, or over the whole
- * vocabulary (top_k = 0); temperature <= 0: greedy, p = 1 at the arg-max.  q: the draft's probabilities, draft_probs fp32 [rows, vocab] (rows of last rows are not read), or 1 at the
+ * vocabulary (top_k = 0); temperature 1e-6 .. 1e6, or <= 0: greedy, p = 1 at the arg-max.  q: the draft's probabilities, draft_probs fp32 [rows, vocab] (rows of last rows are not read), or 1 at the
  * draft where draft_probs = 0 (drafts that were not drawn).  Logits of -infinity or NaN have probability 0.
  *   Row by row a draft x stands while  u_accept[row] * q(x) < p(x)  (greedy: while it is the arg-max).  The first row that does not stand, or the last one, gives the token: the
  * first one, by index (top_k: by rank), at which the running sum of weights exceeds u_pick[r] times the whole, weights max(p - q, 0), at the last row p (and where the former are all

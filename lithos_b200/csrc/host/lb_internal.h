@@ -199,6 +199,7 @@ int lb_driver_load(char* err, size_t errlen); /* LB_OK or LB_ERR_NO_DRIVER */
     X(ssm_tc_local)                   \
     X(ssm_finish)                     \
     X(vd_rows)                        \
+    X(vd_rows_greedy)                 \
     X(vd_rows_topk)                   \
     X(vd_pick_short)                  \
     X(vd_pick)                        \

@@ -37,6 +37,47 @@ __device__ __forceinline__ bool vd_better(float v, int i, float bv, int bi) { re
 // exp((l - max) / T) in 64 bits; an infinite maximum leaves those that share it, -infinity and NaN count as no logit
 __device__ __forceinline__ double vd_exp(float l, float max, double inv_t) { return !(l > -INFINITY) ? 0.0 : l == max ? 1.0 : l < max ? exp(((double)l - (double)max) * inv_t) : 0.0; }
 
+__device__ __forceinline__ float vd_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// a finite float as a double, by its bits (conversions run at a quarter of the rate): 0 and denormal ones come out as some number below 2^-126
+__device__ __forceinline__ double vd_double(float v) {
+    const uint32_t b = __float_as_uint(v);
+    return __hiloint2double((((int)b >> 3) & (int)0x8fffffffu) + 0x38000000, (int)(b << 29));
+}
+
+// exp of many differences l - max in 64 bits: y = (l - max) 256 / (T ln 2) = 256 a + j + f with |f| <= 1/2, exp = 2^a 2^(j/256) e^(f ln 2 / 256), the last factor by its series, whose
+// fourth term is below 2e-13.  Eight operations in 64 bits, which are what the pick's time goes into; the library's exp also serves arguments that do not occur here
+// and makes it twice as long.
+#define VD_STEPS 256
+struct vd_exps {
+    double scale, less; // y = l * scale - less
+    const double* table;
+    float low;          // what lies below adds nothing (2^-1000); a NaN where there is no logit at all
+    __device__ __forceinline__ static void fill(double* table) { // a barrier follows
+        for (int i = threadIdx.x; i < VD_STEPS; i += blockDim.x) table[i] = exp2((double)i / VD_STEPS);
+    }
+    __device__ __forceinline__ vd_exps(const double* t, float max, double temperature) : table(t) {
+        const bool infinite = max == INFINITY; // those that share it have exp = 1
+        scale = infinite ? 0.0 : VD_STEPS * VD_LOG2E / temperature;
+        less = infinite ? 0.0 : (double)max * scale;
+        low = infinite ? max : max > -INFINITY ? (float)fmax((double)max - 693.0 * temperature, -3.4028234e38) : NAN;
+    }
+    __device__ __forceinline__ double operator()(float l) const {
+        constexpr double L = 0.69314718055994530942 / VD_STEPS, magic = 6755399441055744.0; // 1.5 * 2^52: what is added to it is rounded to a whole number
+        const double y = fma(vd_double(l), scale, -less), whole = y + magic, f = y - (whole - magic);
+        double e = fma(f, L * L * L / 6.0, L * L / 2.0);
+        e = fma(f, e, L);
+        e = fma(f, e, 1.0);
+        const int n = __double2loint(whole);
+        e *= table[n & (VD_STEPS - 1)];
+        return l >= low ? __hiloint2double(__double2hiint(e) + ((n >> 8) << 20), __double2loint(e)) : 0.0; // a NaN is not
+    }
+};
+
 // Whether the row's draft stands, and the target's probability of it (from thread 0).  px: that probability
 __device__ __forceinline__ void vd_decide(const lb_vd_params& p, int row, bool last, double px, lb_vd_row st) {
     const int x = p.drafts[row];
@@ -52,66 +93,84 @@ __device__ __forceinline__ void vd_decide(const lb_vd_params& p, int row, bool l
     if (p.p_out) p.p_out[row] = (float)px;
 }
 
-// Rows over the whole vocabulary: maximum, its first index, sum of exponentials.  grid (rows, cluster)
-extern "C" __global__ void __launch_bounds__(VD_THREADS) vd_rows(const __grid_constant__ lb_vd_params p) {
+// f(four logits, index of the first) over a thread's share of logits a..b-1 of x, a % 4 == 0; what lies behind b comes as -infinity
+template <int THREADS, class F>
+__device__ __forceinline__ void vd_each(const float* x, int a, int b, F f) {
+    int i = a + 4 * threadIdx.x;
+    if ((((size_t)x + 4 * (size_t)a) & 15) == 0) {
+        for (; i + 12 * THREADS + 3 < b; i += 16 * THREADS) {
+            float4 v[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) v[h] = __ldg(reinterpret_cast<const float4*>(x + i + 4 * h * THREADS));
+#pragma unroll
+            for (int h = 0; h < 4; ++h) f(v[h], i + 4 * h * THREADS);
+        }
+        for (; i + 3 < b; i += 4 * THREADS) f(__ldg(reinterpret_cast<const float4*>(x + i)), i);
+    }
+    for (; i < b; i += 4 * THREADS) {
+        float4 v = make_float4(x[i], -INFINITY, -INFINITY, -INFINITY);
+        if (i + 1 < b) v.y = x[i + 1];
+        if (i + 2 < b) v.z = x[i + 2];
+        if (i + 3 < b) v.w = x[i + 3];
+        f(v, i);
+    }
+}
+
+// Rows over the whole vocabulary.  Greedy: maximum and its first index; else maximum and sum of exponentials.  The sum is one of 2^(l k - c), k = log2(e) / T, against a reference c that
+// only moves when an exponent would pass 2^24: a multiply-add, an exponential, an addition and a maximum per logit.  What the row's sum is in the end is told
+// in exponents of 2^(max k), with c known exactly.  Where that is not good enough (a NaN among the logits, infinities, exponents beyond 2^24) the sum is taken again with
+// differences from the maximum.  grid (rows, cluster)
+template <bool GREEDY>
+__device__ __forceinline__ void vd_rows_body(const lb_vd_params& p) {
     __shared__ float sm[VD_WARPS + LB_VD_CLUSTER];
     __shared__ int si[VD_WARPS + LB_VD_CLUSTER];
     __shared__ double ss[VD_WARPS + LB_VD_CLUSTER];
     cg::cluster_group cluster = cg::this_cluster();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, row = blockIdx.x, C = gridDim.y, rank = blockIdx.y;
     pdl_wait();
+    const float* x = p.logits + (size_t)row * p.V;
+    const int per = (((p.V + C - 1) / C) + 3) & ~3, a = min(p.V, rank * per), b = min(p.V, a + per);
+    const float k = GREEDY ? 0.f : (float)(VD_LOG2E / p.temperature);
+    float m = -INFINITY, sum = 0.f;
+    double ref = 0.0; // the sum's reference
+    int best = 0x7fffffff;
+    if (GREEDY) {
+        vd_each<VD_THREADS>(x, a, b, [&](const float4& v, int i) {
+            const float mx = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+            if (mx > m) { // the first of them: index order within a thread
+                m = mx;
+                best = v.x == mx ? i : v.y == mx ? i + 1 : v.z == mx ? i + 2 : i + 3;
+            }
+        });
+    } else {
+        float s[2] = {0.f, 0.f}, c = 0.f;
+        vd_each<VD_THREADS>(x, a, b, [&](const float4& v, int) {
+            const float mx = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+            if (mx > m) {
+                const float now = fmaxf(-3.4e38f, mx * k), d = c - now;
+                if (m == -INFINITY || d < -24.f) { // 2^24 times 2^24 logits fit fp32
+                    s[0] *= m == -INFINITY ? 0.f : vd_exp2(d);
+                    s[1] *= m == -INFINITY ? 0.f : vd_exp2(d);
+                    c = now;
+                }
+                m = mx;
+            }
+            s[0] += vd_exp2(fmaf(v.x, k, -c)) + vd_exp2(fmaf(v.y, k, -c));
+            s[1] += vd_exp2(fmaf(v.z, k, -c)) + vd_exp2(fmaf(v.w, k, -c));
+        });
+        sum = s[0] + s[1];
+        ref = (double)c;
+        if (!(sum < INFINITY) || !(fabsf(m * k) < 16777216.f)) { // NaN logits; infinite ones, of which only those that share the maximum count; a c that is known to whole numbers only
+            sum = 0.f;
+            ref = (double)m * (double)k;
+            auto one = [&](float l) { return l == m ? 1.f : l < m ? vd_exp2((l - m) * k) : 0.f; };
+            vd_each<VD_THREADS>(x, a, b, [&](const float4& v, int) { sum += one(v.x) + one(v.y) + one(v.z) + one(v.w); });
+        }
+        if (m == -INFINITY) sum = 0.f;
+    }
     const vd_place at = vd_find(p, row);
     if (!at.covered) return; // the same for the whole cluster
     cluster.barrier_arrive(); // waited for before the first word to another CTA
-    const float* x = p.logits + (size_t)row * p.V;
-    const int per = (((p.V + C - 1) / C) + 3) & ~3, a = min(p.V, rank * per), b = min(p.V, a + per);
-    const float k = p.temperature > 0.0 ? (float)(VD_LOG2E / p.temperature) : 0.f;
-    float m = -INFINITY, sum = 0.f;
-    int best = 0x7fffffff;
-    auto take = [&](const float (&v)[8], const int (&id)[8]) { // index order within a thread
-        float mx = m;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (v[j] > mx) { mx = v[j]; best = id[j]; }
-        if (mx > m) {
-            sum *= exp2f((m - mx) * k);
-            m = mx;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum += v[j] == m ? 1.f : v[j] < m ? exp2f((v[j] - m) * k) : 0.f;
-    };
-    if ((((size_t)x + 4 * (size_t)a) & 15) == 0) {
-        for (int i0 = a + 4 * t; i0 < b; i0 += 8 * VD_THREADS) {
-            float v[8];
-            int id[8];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int i = i0 + 4 * h * VD_THREADS;
-                float4 f = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                if (i + 3 < b) f = __ldg(reinterpret_cast<const float4*>(x + i));
-                else {
-                    if (i < b) f.x = x[i];
-                    if (i + 1 < b) f.y = x[i + 1];
-                    if (i + 2 < b) f.z = x[i + 2];
-                }
-                v[4 * h] = f.x; v[4 * h + 1] = f.y; v[4 * h + 2] = f.z; v[4 * h + 3] = f.w;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) id[4 * h + j] = i + j;
-            }
-            take(v, id);
-        }
-    } else {
-        for (int i0 = a + t; i0 < b; i0 += 8 * VD_THREADS) {
-            float v[8];
-            int id[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                id[j] = i0 + j * VD_THREADS;
-                v[j] = id[j] < b ? x[id[j]] : -INFINITY;
-            }
-            take(v, id);
-        }
-    }
     // the CTA's, then the cluster's: maxima first, then the sums brought to it
     float M = m;
     int I = best;
@@ -123,19 +182,26 @@ extern "C" __global__ void __launch_bounds__(VD_THREADS) vd_rows(const __grid_co
     }
     if (lane == 0) { sm[warp] = M; si[warp] = I; }
     __syncthreads();
-    M = sm[0];
-    I = si[0];
-    for (int w = 1; w < VD_WARPS; ++w)
-        if (vd_better(sm[w], si[w], M, I)) { M = sm[w]; I = si[w]; }
-    double S = sum > 0.f ? (double)sum * (double)(m == M ? 1.f : exp2f((m - M) * k)) : 0.0;
+    M = sm[lane & (VD_WARPS - 1)];
+    I = si[lane & (VD_WARPS - 1)];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
-    if (lane == 0) ss[warp] = S;
-    __syncthreads();
+    for (int o = VD_WARPS / 2; o > 0; o >>= 1) {
+        const float ov = __shfl_xor_sync(0xffffffffu, M, o);
+        const int oi = __shfl_xor_sync(0xffffffffu, I, o);
+        if (vd_better(ov, oi, M, I)) { M = ov; I = oi; }
+    }
+    double S = 0.0;
+    if (!GREEDY) {
+        if (sum > 0.f) S = M == INFINITY ? (m == M ? (double)sum : 0.0) : (double)sum * exp2(ref - (double)M * (double)k);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
+        if (lane == 0) ss[warp] = S;
+        __syncthreads();
+    }
     cluster.barrier_wait();
     if (t == 0) {
         S = 0.0;
-        for (int w = 0; w < VD_WARPS; ++w) S += ss[w];
+        for (int w = 0; w < VD_WARPS && !GREEDY; ++w) S += ss[w];
         *cluster.map_shared_rank(&sm[VD_WARPS + rank], 0) = M;
         *cluster.map_shared_rank(&si[VD_WARPS + rank], 0) = I;
         *cluster.map_shared_rank(&ss[VD_WARPS + rank], 0) = S;
@@ -147,159 +213,189 @@ extern "C" __global__ void __launch_bounds__(VD_THREADS) vd_rows(const __grid_co
         for (int w = 1; w < C; ++w)
             if (vd_better(sm[VD_WARPS + w], si[VD_WARPS + w], M, I)) { M = sm[VD_WARPS + w]; I = si[VD_WARPS + w]; }
         S = 0.0;
-        for (int w = 0; w < C; ++w) {
+        for (int w = 0; w < C && !GREEDY; ++w) {
             const float o = sm[VD_WARPS + w];
             if (ss[VD_WARPS + w] > 0.0) S += ss[VD_WARPS + w] * (o == M ? 1.0 : exp2(((double)o - (double)M) * (double)k));
         }
-        lb_vd_row st = {S, M, I == 0x7fffffff ? 0 : I, 0, 0};
+        const lb_vd_row st = {S, M, I == 0x7fffffff ? 0 : I, 0, 0};
         const int d = p.drafts[row];
         double px = 0.0;
-        if (d >= 0 && d < p.V) px = p.temperature > 0.0 ? (S > 0.0 ? vd_exp(x[d], M, 1.0 / p.temperature) / S : 0.0) : (d == st.best && M > -INFINITY ? 1.0 : 0.0);
+        if (d >= 0 && d < p.V) px = GREEDY ? (d == st.best && M > -INFINITY ? 1.0 : 0.0) : S > 0.0 ? vd_exp(x[d], M, 1.0 / p.temperature) / S : 0.0;
         vd_decide(p, row, at.last, px, st);
     }
 }
+extern "C" __global__ void __launch_bounds__(VD_THREADS, 3) vd_rows(const __grid_constant__ lb_vd_params p) { vd_rows_body<false>(p); }
+extern "C" __global__ void __launch_bounds__(VD_THREADS, 3) vd_rows_greedy(const __grid_constant__ lb_vd_params p) { vd_rows_body<true>(p); }
 
 // ---- rows over the top_k largest ------------------------------------------------------------------------------------------------------------
-#define VT_THREADS 1024
-#define VT_EACH 32   // logits a thread holds
-#define VT_CAND 1024 // candidates that are sorted at once
-// a float's bits in an order that unsigned numbers have; 0 stands for -infinity and NaN, which are no candidates
+#define VT_THREADS 512
+#define VT_CAND 512   // candidates that are ranked at once
+#define VT_GROUPS 256 // groups of threads whose maxima give the bound
+// a float's bits in an order that unsigned numbers have; what is not above 0 stands for -infinity and NaN, which are no candidates
 __device__ __forceinline__ uint32_t vt_key(float v) {
-    if (!(v > -INFINITY)) return 0u;
-    const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v); // -0 = 0
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const uint32_t b = __float_as_uint(fmaxf(v, -INFINITY) + 0.f); // -0 = 0
+    return (b ^ (uint32_t)((int)b >> 31 | (int)0x80000000u)) - 0x007fffffu;
 }
-__device__ __forceinline__ float vt_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
+__device__ __forceinline__ float vt_value(uint32_t key) {
+    key += 0x007fffffu;
+    return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+__device__ __forceinline__ unsigned long long vt_pack(uint32_t key, int i) { return (unsigned long long)key << 32 | (0xffffffffu - (uint32_t)i); }
 
-// VT_CAND numbers in shared memory, descending
-__device__ __forceinline__ void vt_sort(unsigned long long* s) {
+// The K largest of n different numbers (n <= VT_CAND) in descending order, the rest of `out` 0: a number's place is how many are larger
+__device__ __forceinline__ void vt_rank(const unsigned long long* in, int n, unsigned long long* out, int K) {
     const int t = threadIdx.x;
-    unsigned long long v = s[t];
-    for (int size = 2; size <= VT_CAND; size <<= 1)
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-            unsigned long long o;
-            if (stride >= 32) {
-                __syncthreads();
-                s[t] = v;
-                __syncthreads();
-                o = s[t ^ stride];
-            } else o = __shfl_xor_sync(0xffffffffu, v, stride);
-            const bool down = (t & size) == 0, lower = (t & stride) == 0; // this place keeps the larger one
-            v = (down == lower) == (v > o) ? v : o;
-        }
+    if (t < K) out[t] = 0ull;
     __syncthreads();
-    s[t] = v;
+    if (t < n) {
+        const unsigned long long mine = in[t];
+        int place = 0;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) place += in[i] > mine;
+        if (place < K && mine) out[place] = mine;
+    }
+    __syncthreads();
+}
+// the same of C lists of K in descending order: what is larger in another list is found by halving
+__device__ __forceinline__ void vt_merge(const unsigned long long* in, int C, unsigned long long* out, int K) {
+    const int t = threadIdx.x;
+    if (t < K) out[t] = 0ull;
+    __syncthreads();
+    if (t < C * K) {
+        const unsigned long long mine = in[t];
+        int place = t % K;
+        for (int c = 0; c < C; ++c) {
+            if (c == t / K) continue;
+            int lo = 0, hi = K; // the first place whose number is not larger
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (in[c * K + mid] > mine) lo = mid + 1;
+                else hi = mid;
+            }
+            place += lo;
+        }
+        if (place < K && mine) out[place] = mine;
+    }
     __syncthreads();
 }
 
-// The rows' top_k candidates in order (larger logit, then smaller index), as lb_sample_topk takes them.  A thread holds VT_EACH logits; the k-th largest of the threads' maxima
-// bounds the k-th largest from below, and what reaches it is sorted: about k.  Where more than VT_CAND reach it (many equal ones, or a few threads with all of the large ones) the
-// exact bound is found by halving, first of the value, then of the index among the equal ones.  grid (rows, cluster)
-extern "C" __global__ void __launch_bounds__(VT_THREADS) vd_rows_topk(const __grid_constant__ lb_vd_params p) {
-    __shared__ unsigned long long cand[VT_CAND];
+// The rows' top_k candidates in order (larger logit, then smaller index), as lb_sample_topk takes them.  The K-th largest of the maxima of pairs of threads bounds the K-th
+// largest from below; what reaches it is collected in a second pass, from L2, and ranked: K and a few.  Where more than VT_CAND reach it (many equal ones, or a few threads
+// with all of the large ones) the exact bound is found by halving, first of the value, then of the index among the equal ones, a pass each.  grid (rows, cluster)
+extern "C" __global__ void __launch_bounds__(VT_THREADS, 3) vd_rows_topk(const __grid_constant__ lb_vd_params p) {
+    __shared__ unsigned long long cand[VT_CAND], best[LB_VD_TOPK];
     __shared__ unsigned long long from[LB_VD_CLUSTER * LB_VD_TOPK]; // the cluster's lists, at its first CTA
+    __shared__ uint32_t tops[VT_GROUPS], s_bound;
     __shared__ int n_cand;
     cg::cluster_group cluster = cg::this_cluster();
-    const int t = threadIdx.x, row = blockIdx.x, C = gridDim.y, rank = blockIdx.y, K = p.top_k;
+    const int t = threadIdx.x, lane = t & 31, row = blockIdx.x, C = gridDim.y, rank = blockIdx.y, K = p.top_k;
     pdl_wait();
+    const float* x = p.logits + (size_t)row * p.V;
+    const int per = (((p.V + C - 1) / C) + 3) & ~3, a = min(p.V, rank * per), b = min(p.V, a + per);
+    // f(logit, index) over this thread's share of the range
+    auto each = [&](auto f) {
+        vd_each<VT_THREADS>(x, a, b, [&](const float4& v, int i) { f(v.x, i); f(v.y, i + 1); f(v.z, i + 2); f(v.w, i + 3); });
+    };
+    float top = -INFINITY;
+    each([&](float v, int) { top = fmaxf(top, v); });
     const vd_place at = vd_find(p, row);
     if (!at.covered) return;
     cluster.barrier_arrive();
-    const float* x = p.logits + (size_t)row * p.V;
-    const int per = (p.V + C - 1) / C, a = min(p.V, rank * per), b = min(p.V, a + per);
-    cand[t] = 0ull;
+    const float pair = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    if ((t & 1) == 0) tops[t >> 1] = vt_key(pair);
+    if (t == 0) n_cand = 0;
     __syncthreads();
-    for (int base = a; base < b; base += VT_THREADS * VT_EACH) { // the list so far is in cand[0 .. K)
-        uint32_t key[VT_EACH], top = 0u;
+    if (t < 32) { // the largest 20-bit bound that K of the maxima reach; 0: fewer than K do, all candidates count
+        uint32_t g[VT_GROUPS / 32], bound = 0u;
 #pragma unroll
-        for (int j = 0; j < VT_EACH; ++j) {
-            const int i = base + j * VT_THREADS + t;
-            key[j] = i < b ? vt_key(__ldg(x + i)) : 0u;
+        for (int i = 0; i < VT_GROUPS / 32; ++i) g[i] = tops[i * 32 + lane];
+        for (int bit = 31; bit >= 12; --bit) {
+            const uint32_t trial = bound | 1u << bit;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < VT_GROUPS / 32; ++i) n += g[i] >= trial;
+            if ((int)__reduce_add_sync(0xffffffffu, n) >= K) bound = trial;
         }
-#pragma unroll
-        for (int j = 0; j < VT_EACH; ++j) top = max(top, key[j]);
-        // the largest bound that K of the threads' maxima reach (0: fewer than K do, all candidates count)
-        uint32_t bound = 0u;
+        if (lane == 0) s_bound = max(bound, 1u);
+    }
+    __syncthreads();
+    uint32_t bound = s_bound;
+    auto collect = [&](int last) { // those above the bound, and of those equal to it the ones up to index `last`
+        const float low = vt_value(bound);
+        if (top >= low)
+            each([&](float v, int i) {
+                if (v > low || (v == low && i <= last)) {
+                    const int o = atomicAdd(&n_cand, 1);
+                    if (o < VT_CAND) cand[o] = vt_pack(vt_key(v), i);
+                }
+            });
+        __syncthreads();
+    };
+    collect(0x7fffffff);
+    if (n_cand > VT_CAND) { // what lies behind the range comes as -infinity, whose key is 0
+        auto count = [&](auto f) { // over all of the CTA's logits
+            int n = 0;
+            each([&](float v, int i) { n += f(vt_key(v), i); });
+            __syncthreads();
+            if (t == 0) n_cand = 0;
+            __syncthreads();
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (lane == 0 && n) atomicAdd(&n_cand, n);
+            __syncthreads();
+            return n_cand;
+        };
+        bound = 0u;
         for (int bit = 31; bit >= 0; --bit) {
             const uint32_t trial = bound | 1u << bit;
-            if (__syncthreads_count(top >= trial) >= K) bound = trial;
+            if (count([&](uint32_t k, int) { return k >= trial; }) >= K) bound = trial;
         }
-        const uint32_t before = (uint32_t)(cand[K - 1] >> 32); // nothing below the list's end comes in
-        if (before > bound) bound = before;
-        if (bound == 0u) bound = 1u;
-        uint32_t last = 0xffffffffu; // of those equal to the bound: indices up to this one
-        int mine = 0;
-#pragma unroll
-        for (int j = 0; j < VT_EACH; ++j) mine += key[j] >= bound;
-        if (t == 0) n_cand = K;
-        __syncthreads();
-        if (mine) atomicAdd(&n_cand, mine);
-        __syncthreads();
-        if (n_cand > VT_CAND) {
-            auto count = [&](auto f) { // over all of the CTA's logits
-                int n = 0;
-#pragma unroll
-                for (int j = 0; j < VT_EACH; ++j) n += f(key[j], (uint32_t)(base + j * VT_THREADS + t));
-                __syncthreads();
-                if (t == 0) n_cand = 0;
-                __syncthreads();
-                n = __reduce_add_sync(0xffffffffu, n);
-                if ((t & 31) == 0 && n) atomicAdd(&n_cand, n);
-                __syncthreads();
-                return n_cand;
-            };
-            bound = 0u;
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t trial = bound | 1u << bit;
-                if (count([&](uint32_t k, uint32_t) { return k >= trial; }) >= K) bound = trial;
-            }
-            const int above = count([&](uint32_t k, uint32_t) { return k > bound; });
-            last = 0u; // the smallest index with K - above equal ones up to it
-            for (int bit = 30; bit >= 0; --bit) {
-                const uint32_t trial = last | 1u << bit;
-                if (count([&](uint32_t k, uint32_t i) { return k == bound && i < trial; }) < K - above) last = trial;
-            }
+        const int above = count([&](uint32_t k, int) { return k > bound; });
+        int last = 0; // the smallest index with K - above equal ones up to it
+        for (int bit = 24; bit >= 0; --bit) {
+            const int trial = last | 1 << bit;
+            if (count([&](uint32_t k, int i) { return k == bound && i < trial; }) < K - above) last = trial;
         }
         __syncthreads();
-        if (t >= K) cand[t] = 0ull;
-        if (t == 0) n_cand = K;
+        if (t == 0) n_cand = 0;
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < VT_EACH; ++j) {
-            const uint32_t i = (uint32_t)(base + j * VT_THREADS + t);
-            if (key[j] > bound || (key[j] == bound && i <= last)) {
-                const int o = atomicAdd(&n_cand, 1);
-                if (o < VT_CAND) cand[o] = (unsigned long long)key[j] << 32 | (0xffffffffu - i);
-            }
-        }
-        __syncthreads();
-        vt_sort(cand);
+        collect(last);
     }
+    vt_rank(cand, n_cand, best, K);
     cluster.barrier_wait();
-    if (t < K) cluster.map_shared_rank(from, 0)[rank * K + t] = cand[t];
+    __syncthreads();
+    if (t < K) cluster.map_shared_rank(from, 0)[rank * K + t] = best[t];
     cluster.sync();
     if (rank) return;
-    cand[t] = t < C * K ? from[t] : 0ull;
-    __syncthreads();
-    if (C > 1) vt_sort(cand);
-    double* e = reinterpret_cast<double*>(from);
-    const float top = cand[0] ? vt_value((uint32_t)(cand[0] >> 32)) : -INFINITY;
+    if (C > 1) vt_merge(from, C, best, K);
+    double* e = reinterpret_cast<double*>(cand);
+    const float first = best[0] ? vt_value((uint32_t)(best[0] >> 32)) : -INFINITY;
     if (t < K) {
-        const float v = vt_value((uint32_t)(cand[t] >> 32));
-        e[t] = cand[t] ? vd_exp(v, top, 1.0 / p.temperature) : 0.0;
+        const float v = vt_value((uint32_t)(best[t] >> 32));
+        e[t] = best[t] ? vd_exp(v, first, 1.0 / p.temperature) : 0.0;
         p.list_val[(size_t)row * LB_VD_TOPK + t] = v;
-        p.list_idx[(size_t)row * LB_VD_TOPK + t] = (int)(0xffffffffu - (uint32_t)cand[t]);
+        p.list_idx[(size_t)row * LB_VD_TOPK + t] = (int)(0xffffffffu - (uint32_t)best[t]);
     }
     __syncthreads();
-    if (t == 0) {
-        lb_vd_row st = {0.0, top, cand[0] ? (int)(0xffffffffu - (uint32_t)cand[0]) : 0, 0, 0};
-        double px = 0.0;
+    if (t < 32) { // the sum, and the draft's place, by one warp
         const int d = p.drafts[row];
-        for (; st.n < K && cand[st.n]; ++st.n) {
-            st.z += e[st.n];
-            if ((int)(0xffffffffu - (uint32_t)cand[st.n]) == d) px = e[st.n];
+        double z = 0.0, px = 0.0;
+        int n = 0;
+        for (int i = lane; i < K; i += 32) {
+            if (!best[i]) continue;
+            ++n;
+            z += e[i];
+            if ((int)(0xffffffffu - (uint32_t)best[i]) == d) px = e[i];
         }
-        vd_decide(p, row, at.last, st.z > 0.0 ? px / st.z : 0.0, st);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            z += __shfl_xor_sync(0xffffffffu, z, o);
+            px += __shfl_xor_sync(0xffffffffu, px, o); // one lane's, the others' 0
+        }
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (t == 0) {
+            const lb_vd_row st = {z, first, best[0] ? (int)(0xffffffffu - (uint32_t)best[0]) : 0, 0, n};
+            vd_decide(p, row, at.last, z > 0.0 ? px / z : 0.0, st);
+        }
     }
 }
 
@@ -332,57 +428,63 @@ __device__ __forceinline__ void vd_write(const lb_vd_params& p, int r, int first
     if (threadIdx.x == 0) p.accepted[r] = at - first;
 }
 
-// Greedy, or from the rows' lists: one CTA of LB_VD_TOPK threads per request
-extern "C" __global__ void __launch_bounds__(LB_VD_TOPK) vd_pick_short(const __grid_constant__ lb_vd_params p) {
-    __shared__ double w[LB_VD_TOPK];
-    __shared__ int token;
-    const int t = threadIdx.x, r = blockIdx.x;
+// Greedy, or from the rows' lists: a warp per request, a lane two neighbouring ranks
+extern "C" __global__ void __launch_bounds__(32) vd_pick_short(const __grid_constant__ lb_vd_params p) {
+    const int lane = threadIdx.x, r = blockIdx.x;
     pdl_wait();
     int first, last;
     const int at = vd_stop(p, r, first, last);
     if (at < 0) return;
     const lb_vd_row st = p.stat[at];
-    if (t == 0) token = st.best;
-    if (p.temperature > 0.0) {
-        const int idx = t < st.n ? p.list_idx[(size_t)at * LB_VD_TOPK + t] : -1;
-        double e = 0.0, left = 0.0;
-        if (t < st.n) {
-            e = vd_exp(p.list_val[(size_t)at * LB_VD_TOPK + t], st.max, 1.0 / p.temperature) / st.z;
-            left = e;
-            if (at < last) {
-                const double q = p.probs ? (double)p.probs[(size_t)at * p.V + idx] : idx == p.drafts[at] ? 1.0 : 0.0;
-                left = q > 0.0 ? fmax(e - q, 0.0) : e;
+    int token = st.best;
+    if (p.temperature > 0.0 && st.n) {
+        double e[2], w[2];
+        int idx[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 2 * lane + j;
+            idx[j] = i < st.n ? p.list_idx[(size_t)at * LB_VD_TOPK + i] : -1;
+            e[j] = w[j] = 0.0;
+            if (i < st.n) {
+                e[j] = w[j] = vd_exp(p.list_val[(size_t)at * LB_VD_TOPK + i], st.max, 1.0 / p.temperature) / st.z;
+                if (at < last) {
+                    const double q = p.probs ? (double)p.probs[(size_t)at * p.V + idx[j]] : idx[j] == p.drafts[at] ? 1.0 : 0.0;
+                    if (q > 0.0) w[j] = fmax(e[j] - q, 0.0);
+                }
             }
         }
-        if (!__syncthreads_or(left > 0.0)) left = e; // rounding left nothing
-        w[t] = left;
-        __syncthreads();
-        if (t == 0 && st.n) {
-            double total = 0.0, sum = 0.0;
-            for (int i = 0; i < st.n; ++i) total += w[i];
-            const double goal = (double)p.u_pick[r] * total;
-            int i = 0, pick = 0;
-            for (; i < st.n; ++i) {
-                sum += w[i];
-                if (w[i] > 0.0) pick = i;
-                if (sum > goal) break;
-            }
-            token = p.list_idx[(size_t)at * LB_VD_TOPK + pick];
+        if (!__any_sync(0xffffffffu, w[0] > 0.0 || w[1] > 0.0)) { // rounding left nothing
+            w[0] = e[0];
+            w[1] = e[1];
         }
+        double run = w[0] + w[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double v = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += v;
+        }
+        const double goal = (double)p.u_pick[r] * __shfl_sync(0xffffffffu, run, 31), half = run - w[1];
+        const bool hit0 = w[0] > 0.0 && half > goal, hit1 = w[1] > 0.0 && run > goal;
+        const uint32_t hit = __ballot_sync(0xffffffffu, hit0 || hit1), some = __ballot_sync(0xffffffffu, w[0] > 0.0 || w[1] > 0.0);
+        // the first lane behind the goal; none: the last with weight
+        const int lane_of = hit ? __ffs(hit) - 1 : 31 - __clz(some);
+        token = __shfl_sync(0xffffffffu, (hit ? hit0 : !(w[1] > 0.0)) ? idx[0] : idx[1], lane_of);
     }
-    __syncthreads();
     vd_write(p, r, first, last, at, token);
 }
 
-// From the whole vocabulary: a cluster per request, its CTAs and their warps taking neighbouring ranges in index order.  grid (requests, cluster)
-#define VP_THREADS 1024
-#define VP_WARPS 32
-extern "C" __global__ void __launch_bounds__(VP_THREADS) vd_pick(const __grid_constant__ lb_vd_params p) {
+// From the whole vocabulary: a cluster per request, its CTAs and their warps taking neighbouring ranges in index order.  Against certain drafts, and in a last row, the weights are
+// exponentials as they are (one pass); against the draft's probabilities they have to be divided by their sum first (a pass for it).  grid (requests, cluster)
+#define VP_THREADS 512
+#define VP_WARPS (VP_THREADS / 32)
+extern "C" __global__ void __launch_bounds__(VP_THREADS, 2) vd_pick(const __grid_constant__ lb_vd_params p) {
     __shared__ double part[2];           // this CTA's sum: of the exponentials, of the weights
-    __shared__ double ws[VP_WARPS];
-    __shared__ int s_token;
+    __shared__ double ws[VP_WARPS], table[VD_STEPS];
+    __shared__ int s_token, s_last;
     cg::cluster_group cluster = cg::this_cluster();
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, r = blockIdx.x, C = gridDim.y, rank = blockIdx.y;
+    vd_exps::fill(table);
+    __syncthreads();
     pdl_wait();
     int first, last;
     const int at = vd_stop(p, r, first, last);
@@ -392,63 +494,100 @@ extern "C" __global__ void __launch_bounds__(VP_THREADS) vd_pick(const __grid_co
     const bool inner = at < last;
     const float* q = inner && p.probs ? p.probs + (size_t)at * p.V : nullptr;
     const int gone = inner && !p.probs ? p.drafts[at] : -1; // a certain draft
-    const double inv_t = 1.0 / p.temperature;
+    const vd_exps expo(table, st.max, p.temperature);
     const int per = (p.V + C * VP_WARPS - 1) / (C * VP_WARPS), a = min(p.V, (rank * VP_WARPS + warp) * per), b = min(p.V, a + per); // this warp's range
-    auto all = [&](double v, int which) { // sum over the CTA into part[which] (ws: the warps'), then over the cluster in its order
+    double sums[LB_VD_CLUSTER];
+    auto all = [&](double v, int which) { // sum over the CTA into part[which] (ws: the warps'), then over the cluster in its order; sums: the CTAs'
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         if (lane == 0) ws[warp] = v;
         __syncthreads();
-        if (t == 0) {
-            double s = 0.0;
-            for (int w = 0; w < VP_WARPS; ++w) s += ws[w];
-            part[which] = s;
+        if (warp == 0) {
+            double s = lane < VP_WARPS ? ws[lane] : 0.0;
+#pragma unroll
+            for (int o = VP_WARPS / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (lane == 0) part[which] = s;
         }
         cluster.sync();
         double s = 0.0;
-        for (int c = 0; c < C; ++c) s += *cluster.map_shared_rank(&part[which], c);
+#pragma unroll
+        for (int c = 0; c < LB_VD_CLUSTER; ++c) sums[c] = c < C ? *cluster.map_shared_rank(&part[which], c) : 0.0;
+#pragma unroll
+        for (int c = 0; c < LB_VD_CLUSTER; ++c) s += sums[c];
         return s;
     };
-    double z = 1.0;
-    if (q) {
-        double s = 0.0;
-        for (int i = a + lane; i < b; i += 32) s += vd_exp(x[i], st.max, inv_t);
-        z = 1.0 / all(s, 0);
-    }
-    bool rest = inner;
-    auto weight = [&](int i) {
-        const double e = vd_exp(x[i], st.max, inv_t) * z;
-        if (!rest) return e;
-        if (!q) return i == gone ? 0.0 : e;
-        const float o = q[i];
-        return o > 0.f ? fmax(e - (double)o, 0.0) : e;
+    // f(index, logit) or f(index, logit, q) over a warp's range, eight values of a lane in flight
+    auto over = [&](auto f) {
+        double s0 = 0.0, s1 = 0.0;
+        int i = a + lane;
+        for (; i + 224 < b; i += 256) {
+            float l[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) l[j] = __ldg(x + i + 32 * j);
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                s0 += f(i + 32 * j, l[j]);
+                s1 += f(i + 32 * j + 32, l[j + 1]);
+            }
+        }
+        for (; i < b; i += 32) s0 += f(i, x[i]);
+        return s0 + s1;
     };
-    double s = 0.0;
-    for (int i = a + lane; i < b; i += 32) s += weight(i);
-    double total = all(s, 1);
-    if (rest && !(total > 0.0)) { // rounding left nothing: from p itself
-        rest = false;
+    auto over2 = [&](auto f) {
+        double s0 = 0.0, s1 = 0.0;
+        int i = a + lane;
+        for (; i + 224 < b; i += 256) {
+            float l[8], o[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                l[j] = __ldg(x + i + 32 * j);
+                o[j] = __ldg(q + i + 32 * j);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                s0 += f(l[j], o[j]);
+                s1 += f(l[j + 1], o[j + 1]);
+            }
+        }
+        for (; i < b; i += 32) s0 += f(x[i], q[i]);
+        return s0 + s1;
+    };
+    auto rest = [&](float l, float o) { // max(p - q, 0); a q that is no positive number is 0
+        const double e = expo(l), d = e - vd_double(fmaxf(o, 0.f));
+        return o < INFINITY && __double2hiint(d) >= 0 ? d : o >= 0.f ? 0.0 : e;
+    };
+    auto plain = [&](int, float l) { return expo(l); };
+    auto without = [&](int i, float l) { return i == gone ? 0.0 : expo(l); };
+    double total;
+    bool whole = !inner; // the weights are p
+    if (q) {
+        const double z = 1.0 / all(over(plain), 0);
+        for (int i = t; i < VD_STEPS; i += VP_THREADS) table[i] *= z; // from here on the exponentials are probabilities
+        __syncthreads();
+        total = all(over2(rest), 1);
+    } else total = all(gone >= 0 ? over(without) : over(plain), 1);
+    if (!whole && !(total > 0.0)) { // rounding left nothing: from p itself
+        whole = true;
         cluster.sync(); // the sums have been read
-        s = 0.0;
-        for (int i = a + lane; i < b; i += 32) s += weight(i);
-        total = all(s, 1);
-    }
-    const double goal = (double)p.u_pick[r] * total;
-    double before = 0.0;
-    int owner = 0; // the CTA whose range the goal lies in: the last one with weight where rounding has left it behind them all
-    for (int c = 0; c < C; ++c) {
-        const double v = *cluster.map_shared_rank(&part[1], c);
-        if (!(v > 0.0)) continue;
-        double sum = 0.0;
-        for (int k = 0; k < c; ++k) sum += *cluster.map_shared_rank(&part[1], k);
-        owner = c;
-        before = sum;
-        if (sum + v > goal) break;
+        total = all(over(plain), 1);
     }
     cluster.sync(); // nobody leaves while its sums are read
+    const double goal = (double)p.u_pick[r] * total;
+    double base = 0.0, sum = 0.0;
+    int owner = 0; // the CTA whose range the goal lies in: the last one with weight where rounding has left it behind them all
+    bool found = false;
+#pragma unroll
+    for (int c = 0; c < LB_VD_CLUSTER; ++c) {
+        if (!found && sums[c] > 0.0) {
+            owner = c;
+            base = sum;
+            found = sum + sums[c] > goal;
+        }
+        sum += sums[c];
+    }
     if (rank != owner) return;
     int w0 = 0;
-    double sum = before, base = before;
+    sum = base;
     for (int w = 0; w < VP_WARPS; ++w) {
         if (!(ws[w] > 0.0)) continue;
         w0 = w;
@@ -456,15 +595,25 @@ extern "C" __global__ void __launch_bounds__(VP_THREADS) vd_pick(const __grid_co
         sum += ws[w];
         if (sum > goal) break;
     }
-    // the range of warp w0, one value a thread, 1024 at a time
-    if (t == 0) s_token = -1;
-    __syncthreads();
+    // the range of warp w0, four neighbours a thread, 4 VP_THREADS at a time; s_token the first behind the goal, s_last the last with weight
+    if (t == 0) {
+        s_token = 0x7fffffff;
+        s_last = -1;
+    }
     const int lo = min(p.V, (rank * VP_WARPS + w0) * per), hi = min(p.V, lo + per);
-    int fallback = st.best; // the last token with weight
-    for (int i0 = lo; i0 < hi; i0 += VP_THREADS) {
-        const int i = i0 + t;
-        const double v = i < hi ? weight(i) : 0.0;
-        double run = v;
+    for (int i0 = lo; i0 < hi; i0 += 4 * VP_THREADS) {
+        const int i = i0 + 4 * t;
+        double v[4], run = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j] = 0.0;
+            if (i + j < hi) {
+                const float l = x[i + j];
+                v[j] = whole ? expo(l) : q ? rest(l, q[i + j]) : without(i + j, l);
+            }
+            run += v[j];
+        }
+        const double mine = run;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const double u = __shfl_up_sync(0xffffffffu, run, o);
@@ -473,28 +622,29 @@ extern "C" __global__ void __launch_bounds__(VP_THREADS) vd_pick(const __grid_co
         __syncthreads(); // ws has been read
         if (lane == 31) ws[warp] = run;
         __syncthreads();
-        double add = base;
-        for (int w = 0; w < warp; ++w) add += ws[w];
-        const uint32_t hit = __ballot_sync(0xffffffffu, v > 0.0 && add + run > goal), some = __ballot_sync(0xffffffffu, v > 0.0);
-        __shared__ int s_hit[VP_WARPS], s_some[VP_WARPS];
-        if (lane == 0) {
-            s_hit[warp] = hit ? __ffs(hit) - 1 : -1;
-            s_some[warp] = some ? 31 - __clz(some) : -1;
+        double upto = base + (run - mine), all_of = 0.0;
+        int end = -1;
+        for (int w = 0; w < VP_WARPS; ++w) {
+            if (w < warp) upto += ws[w];
+            all_of += ws[w];
         }
-        __syncthreads();
-        if (t == 0)
-            for (int w = 0; w < VP_WARPS; ++w) {
-                if (s_some[w] >= 0) fallback = i0 + 32 * w + s_some[w];
-                if (s_hit[w] >= 0) {
-                    s_token = i0 + 32 * w + s_hit[w];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            upto += v[j];
+            if (v[j] > 0.0) {
+                if (upto > goal) {
+                    atomicMin(&s_token, i + j);
                     break;
                 }
+                end = i + j;
             }
-        for (int w = 0; w < VP_WARPS; ++w) base += ws[w];
+        }
+        end = __reduce_max_sync(0xffffffffu, end);
+        if (lane == 0) atomicMax(&s_last, end);
+        base += all_of;
         __syncthreads();
-        if (s_token >= 0) break;
+        if (s_token != 0x7fffffff) break;
     }
-    if (t == 0 && s_token < 0) s_token = fallback;
     __syncthreads();
-    vd_write(p, r, first, last, at, s_token);
+    vd_write(p, r, first, last, at, s_token != 0x7fffffff ? s_token : s_last >= 0 ? s_last : st.best);
 }

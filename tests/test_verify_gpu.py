@@ -21,7 +21,7 @@ def case(V, drafts, seed=1, spread=2.0, noise=0.7, temperature=1.0, spare=0):
             "u_accept": rng.random(rows).astype(np.float32), "u_pick": rng.random(len(drafts)).astype(np.float32)}
 
 
-def run(lb, ctx, c, temperature, top_k, probs=True, shift=0, want_p=True):
+def run(lb, ctx, c, temperature, top_k, probs=True, shift=0, want_p=True, tol=2.0 ** -18):
     """the call's results, checked against the plain form"""
     V, n, rows = c["logits"].shape[1], c["n"], c["rows"]
     drafts = c["drafts"] if probs else c["best"]
@@ -37,7 +37,7 @@ def run(lb, ctx, c, temperature, top_k, probs=True, shift=0, want_p=True):
     assert np.array_equal(got[0], want[0])
     # a row's sum is one of 32-bit exponentials: arguments to 2^-23 of themselves, weighted by what they add at most 2^-18 here; the output's rounding 2^-24
     if want_p:
-        assert np.allclose(got[2], want[2], rtol=2.0 ** -18, atol=1e-30)
+        assert np.allclose(got[2], want[2], rtol=tol, atol=1e-30)
     else:
         assert (got[2] == -9).all()
     for b in (*d.values(), tokens, accepted, p_out):
@@ -108,6 +108,18 @@ def test_verify_many_equal_logits(lb, ctx, V):
     run(lb, ctx, c, 1.0, 64, probs=False)
 
 
+@pytest.mark.parametrize("temperature", [1e-6, 0.01, 1e6])
+def test_verify_temperatures(lb, ctx, temperature):
+    """from nearly greedy to uniform; logits far from 0 and far apart"""
+    c = case(5000, [3, 2], seed=19, temperature=1.0)
+    c["logits"][0:4] += np.float32(1e4)
+    c["logits"][5, 10] = np.float32(3e38)
+    c["logits"][6] *= np.float32(1e30)
+    for top_k in (0, 30):
+        run(lb, ctx, c, temperature, top_k, tol=2.0 ** -16)
+        run(lb, ctx, c, temperature, top_k, probs=False, tol=2.0 ** -16)
+
+
 def test_verify_draft_equals_target(lb, ctx):
     """q = p to rounding: drafts stand for every u below 1, and a residue of rounding falls back to p"""
     c = case(500, [3, 3], seed=14, noise=0.0)
@@ -173,7 +185,7 @@ def test_verify_refusals(lb, ctx):
     null, odd = type("At", (), {"ptr": 0}), type("At", (), {"ptr": b.ptr + 2})
     good = [b, 10, b, 1, 2, b, None, b, b, b, b, 1.0, 0, None]
     for i, v in ((0, null), (0, odd), (1, 0), (1, (1 << 24) + 1), (2, null), (3, 0), (3, 257), (4, 0), (4, 8193), (5, null), (6, odd), (7, null), (8, null), (9, null), (10, null),
-                 (11, float("nan")), (11, float("inf")), (12, -1), (12, 65), (13, odd)):
+                 (11, float("nan")), (11, float("inf")), (11, 1e-7), (11, 1e7), (12, -1), (12, 65), (13, odd)):
         a = list(good)
         a[i] = v
         with pytest.raises(lb.LithosError) as e:
