@@ -205,13 +205,9 @@ LB_API int lb_init_images(int device, const char* kernel_dir, const char* images
     c->attn_scratch_bytes = (size_t)8 * 64 * 8 * 260 * sizeof(float) + 256;
     LB_CU(c, lb_drv.MemAlloc(&c->attn_scratch, c->attn_scratch_bytes));
     LB_CU(c, lb_drv.MemsetD8Async(c->attn_scratch, 0, c->attn_scratch_bytes, c->stream));
-    if (c->fn[LBK_kv4_attn_256_1]) {
-        size_t recs = 0; /* two a CTA */
-        for (int mt = 1; mt <= 4; mt *= 2) {
-            const size_t r = (size_t)2 * LB_KV4_CTAS(128, mt) * c->sm_count * LB_KV4_COLS(mt) * LB_KV4_REC(256) * sizeof(float);
-            if (r > recs) recs = r;
-        }
-        LB_CU(c, lb_drv.MemAlloc(&c->kv4_records, recs + 2 * (size_t)c->sm_count * sizeof(lb_kv4_join)));
+    if (c->fn[LBK_kv4_attn_256]) {
+        const size_t ctas = (size_t)LB_KV4_CTAS * c->sm_count, recs = 2 * ctas * LB_KV4_COLS * LB_KV4_REC(256) * sizeof(float);
+        LB_CU(c, lb_drv.MemAlloc(&c->kv4_records, recs + ctas * sizeof(lb_kv4_join)));
         c->kv4_joins = c->kv4_records + recs;
     }
     if (c->fn[LBK_vd_rows]) LB_CU(c, lb_drv.MemAlloc(&c->vd_stat, (size_t)LB_VD_ROWS * (sizeof(lb_vd_row) + LB_VD_TOPK * 8)));

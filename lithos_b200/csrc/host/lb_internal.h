@@ -209,15 +209,9 @@ int lb_driver_load(char* err, size_t errlen); /* LB_OK or LB_ERR_NO_DRIVER */
     X(kv4_read_64)                    \
     X(kv4_read_128)                   \
     X(kv4_read_256)                   \
-    X(kv4_attn_64_1)                  \
-    X(kv4_attn_128_1)                 \
-    X(kv4_attn_256_1)                 \
-    X(kv4_attn_64_2)                  \
-    X(kv4_attn_128_2)                 \
-    X(kv4_attn_256_2)                 \
-    X(kv4_attn_64_4)                  \
-    X(kv4_attn_128_4)                 \
-    X(kv4_attn_256_4)                 \
+    X(kv4_attn_64)                    \
+    X(kv4_attn_128)                   \
+    X(kv4_attn_256)                   \
     X(kv4_merge_64)                   \
     X(kv4_merge_128)                  \
     X(kv4_merge_256)                  \

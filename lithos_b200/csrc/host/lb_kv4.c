@@ -88,24 +88,21 @@ LB_API int lb_kv4_attention(lb_ctx* c, const lb_kv4_cache* cache, const lb_kv4_b
     if (!q || !out || type < 0 || type > 2 || (q | gate) % size_of(type) || (q_norm_w | out) % 2 || head_stride < D || row_stride < 0)
         return lb_fail(c, LB_ERR_INVALID, "lb_kv4_attention: q, gate of an element type (0..2), aligned to it, heads at least dim apart; out");
     LB_TRY(rotation(c, "lb_kv4_attention", D, rot_dims, rope_theta, eps, p.freq));
-    const int G = n_heads / HKV, most_cols = max_new * G, MT = most_cols <= LB_KV4_COLS(1) ? 1 : most_cols <= LB_KV4_COLS(2) ? 2 : 4, sets = (most_cols + LB_KV4_COLS(MT) - 1) / LB_KV4_COLS(MT);
+    const int G = n_heads / HKV, sets = (max_new * G + LB_KV4_COLS - 1) / LB_KV4_COLS;
     p.b.max_new = max_new;
     p.q = (const void*)q; p.gate = (const void*)gate; p.norm_w = (const uint16_t*)q_norm_w; p.out = (uint16_t*)out;
     p.records = (float*)c->kv4_records; p.joins = (lb_kv4_join*)c->kv4_joins;
     p.row_stride = row_stride; p.head_stride = head_stride;
     p.HQ = n_heads; p.type = type; p.rot_dims = rot_dims; p.eps = eps;
     p.wide = ((q | (uint64_t)row_stride * (uint64_t)size_of(type) | (uint64_t)head_stride * (uint64_t)size_of(type)) & 15) == 0;
+    p.out_wide = out % 16 == 0;
     /* no more CTAs than tiles that a full cache would have */
     const int64_t most = (int64_t)batch->n_reqs * HKV * sets * ((cache->max_ctx + LB_KV4_TILE - 1) / LB_KV4_TILE);
-    unsigned ctas = (unsigned)(c->sm_count * LB_KV4_CTAS(D, MT));
-    if ((int64_t)ctas > most) ctas = (unsigned)most;
-    void* params[] = {&p};
-#define KV4_VARIANT(MT) \
-    {by_dim(D, LBK_kv4_attn_64_##MT, LBK_kv4_attn_128_##MT, LBK_kv4_attn_256_##MT), by_dim(D, LB_KV4_SMEM(64, MT), LB_KV4_SMEM(128, MT), LB_KV4_SMEM(256, MT))}
-    const int variants[3][2] = {KV4_VARIANT(1), KV4_VARIANT(2), KV4_VARIANT(4)}, *variant = variants[MT / 2];
-    LB_TRY(lb_launch(c, variant[0], ctas, 1, 1, 256, (unsigned)variant[1], params, 1));
+    int ctas = c->sm_count * LB_KV4_CTAS;
+    if (ctas > most) ctas = (int)most;
+    void* params[] = {&p, &ctas};
+    LB_TRY(lb_launch(c, by_dim(D, LBK_kv4_attn_64, LBK_kv4_attn_128, LBK_kv4_attn_256), (unsigned)ctas, 1, 1, 256,
+                     (unsigned)by_dim(D, LB_KV4_SMEM(64), LB_KV4_SMEM(128), LB_KV4_SMEM(256)), params, 1));
     if (ctas == 1) return LB_OK; /* nothing is cut */
-    int n_ctas = (int)ctas, slots = LB_KV4_COLS(MT);
-    void* mparams[] = {&p, &n_ctas, &slots};
-    return lb_launch(c, by_dim(D, LBK_kv4_merge_64, LBK_kv4_merge_128, LBK_kv4_merge_256), (unsigned)c->sm_count, 1, 1, 1024, 0, mparams, 1);
+    return lb_launch(c, by_dim(D, LBK_kv4_merge_64, LBK_kv4_merge_128, LBK_kv4_merge_256), (unsigned)c->sm_count, 1, 1, 1024, 0, params, 1);
 }

@@ -559,7 +559,6 @@ typedef struct {
 #define LB_KV4_BLOCK(D) (18 * (D))
 #define LB_KV4_REQS 256   /* requests of a batch */
 #define LB_KV4_NEW 16     /* new tokens of a request in an attention call */
-#define LB_KV4_TILE 128   /* rows of a tile: the unit of work of the attention */
 typedef struct {
     unsigned char* cache;
     const int32_t* seqs;   /* [n_reqs] sequence of every request; NULL: request r is sequence r */
@@ -596,14 +595,15 @@ typedef struct {
     int64_t row_stride, head_stride; /* of q and gate, elements */
     int32_t HQ, type, rot_dims, wide;
     float eps;
-    int32_t pad_;
+    int32_t out_wide;       /* out is 16-byte aligned */
     double freq[128];
 } lb_kv4_attn_params;
-/* Columns taken at a time, CTAs per SM and ring stages of the attention kernel's variants.  A CTA uses its shared memory for the ring, queries, probabilities, the rest */
-#define LB_KV4_COLS(MT) (8 * (MT))
-#define LB_KV4_CTAS(D, MT) ((MT) == 1 ? 2 : 1)
-#define LB_KV4_STAGES(D, MT) ((D) == 256 ? ((MT) == 4 ? 3 : (MT) == 2 ? 4 : 2) : (MT) == 1 && (D) == 128 ? 4 : 6)
-#define LB_KV4_SMEM(D, MT) (LB_KV4_STAGES(D, MT) * 8 * LB_KV4_BLOCK(D) + (MT) * (D) * 32 + (MT) * (D) * 64 + 6 * 1024 + (MT) * 2 * 1024)
+/* The attention kernel: columns taken at a time, rows of a tile, CTAs per SM, ring stages.  Shared memory: the ring, probabilities, queries, the rest */
+#define LB_KV4_COLS 8
+#define LB_KV4_TILE 128
+#define LB_KV4_CTAS 2
+#define LB_KV4_STAGES(D) ((D) == 256 ? 2 : (D) == 128 ? 4 : 6)
+#define LB_KV4_SMEM(D) (LB_KV4_STAGES(D) * 8 * LB_KV4_BLOCK(D) + (D) * 96 + 8 * 1024)
 
 /* ---- drafted tokens against the target's probabilities (verify.cu) -------------------------------------------- */
 #define LB_VD_REQS 256
