@@ -97,12 +97,12 @@ LB_API int lb_kv4_attention(lb_ctx* c, const lb_kv4_cache* cache, const lb_kv4_b
     p.wide = ((q | (uint64_t)row_stride * (uint64_t)size_of(type) | (uint64_t)head_stride * (uint64_t)size_of(type)) & 15) == 0;
     p.out_wide = out % 16 == 0;
     /* no more CTAs than tiles that a full cache would have */
-    const int64_t most = (int64_t)batch->n_reqs * HKV * sets * ((cache->max_ctx + LB_KV4_TILE - 1) / LB_KV4_TILE);
-    int ctas = c->sm_count * LB_KV4_CTAS;
+    const int64_t most = (int64_t)batch->n_reqs * HKV * sets * ((cache->max_ctx + LB_KV4_TILE(D) - 1) / LB_KV4_TILE(D));
+    int ctas = c->sm_count * LB_KV4_CTAS < LB_KV4_MAX_CTAS ? c->sm_count * LB_KV4_CTAS : LB_KV4_MAX_CTAS;
     if (ctas > most) ctas = (int)most;
     void* params[] = {&p, &ctas};
     LB_TRY(lb_launch(c, by_dim(D, LBK_kv4_attn_64, LBK_kv4_attn_128, LBK_kv4_attn_256), (unsigned)ctas, 1, 1, 256,
-                     (unsigned)by_dim(D, LB_KV4_SMEM(64), LB_KV4_SMEM(128), LB_KV4_SMEM(256)), params, 1));
+                     LB_KV4_SMEM, params, 1));
     if (ctas == 1) return LB_OK; /* nothing is cut */
-    return lb_launch(c, by_dim(D, LBK_kv4_merge_64, LBK_kv4_merge_128, LBK_kv4_merge_256), (unsigned)c->sm_count, 1, 1, 1024, 0, params, 1);
+    return lb_launch(c, by_dim(D, LBK_kv4_merge_64, LBK_kv4_merge_128, LBK_kv4_merge_256), 2u * (unsigned)c->sm_count, 1, 1, 256, 0, params, 1);
 }

@@ -10,8 +10,8 @@
 //     columns would leave empty.  A query is scaled by a power of two to [2^13, 2^14) at its largest.  Scores, sums and read-outs are fp32, a tile's read-outs added up
 //     by themselves (the products' own additions cut off); the output is fp16, what lb_gemm_int4 takes.
 //   * lowest_t sum(q) is one product more per 8 rows, p_t lowest_t and the sum of p one per 16.
-//   * A tile is 128 rows, one bulk copy, requested by whichever warp is the last to be done with the place it goes to.  A warp does the scores of 16 rows, leaves p scale in shared
-//     memory as operands, and adds up a group's 64 features over its part of the tile.  Probabilities are taken against the largest score, and weights against the largest scale, at
+//   * A tile is 32768 / D rows, 36 KB, one bulk copy, requested by whichever warp is the last to be done with the place it goes to.  A warp does the scores of 256 / D blocks of 16
+//     rows, leaves p scale in shared memory as operands, and adds up a group's 64 features over its part of the tile.  Probabilities are taken against the largest score, and weights against the largest scale, at
 //     the last time that a score passed its reference by 2^6 or a scale by 2^5, which what is left of fp16's range allows; so a tile usually costs one barrier and
 //     no exchange of maxima.
 //   * All tiles of all items are dealt evenly to the CTAs in one line, so that ragged batches balance; an item cut by a border leaves records that kv4_merge joins in order.
@@ -21,12 +21,17 @@
 #define KA_WARPS 8
 #define KA_THREADS (32 * KA_WARPS)
 #define KA_COLS LB_KV4_COLS
-#define KA_TILE LB_KV4_TILE
 
 __device__ __forceinline__ void ka_mma(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// the same onto nothing
+__device__ __forceinline__ void ka_mma0(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t ka_pack(float x, float y) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -52,14 +57,15 @@ struct ka_item { int r, kv, z, tile, tiles; }; // a place in the line of tiles
 
 #define KA_LIFT 4.f  // probabilities are 2^4 at their reference
 #define KA_OVER 6.f  // and may pass it by 2^6
-#define KA_WIDE 0x1400u // a scale may pass its group's reference by 2^5: fp16 bits
+#define KA_WIDE 0x14001400u // a scale may pass its group's reference by 2^5: fp16 bits
 
 template <int D>
 struct ka {
-    static constexpr int S = D / 64, PARTS = KA_WARPS / S, BLK = LB_KV4_BLOCK(D), NS = LB_KV4_STAGES(D);
+    static constexpr int S = D / 64, PARTS = KA_WARPS / S, BLK = LB_KV4_BLOCK(D), NS = LB_KV4_STAGES;
+    static constexpr int BW = 4 / S, TILE = LB_KV4_TILE(D), BLOCKS = TILE / 16; // blocks of a warp; block w + 8 k is warp w's
     struct alignas(128) smem {
-        unsigned char ring[NS][8 * BLK];
-        uint4 p[S][KA_WARPS][32];       // p scale as operands of the products: [group][16 rows of the tile]; an item's sums at its end
+        unsigned char ring[NS][BLOCKS * BLK];
+        uint4 p[S][BLOCKS][32];         // p scale as operands of the products: [group][block of the tile]; an item's sums at its end
         uint4 q[4 * S][32];             // queries likewise: step 4 group + 2 word + u
         uint2 qsum[32];                 // sums of a query's groups as the operand that meets (scale, lowest)
         float part[KA_WARPS][KA_COLS][S + 1];
@@ -72,7 +78,7 @@ struct ka {
         int len[LB_KV4_REQS], n[LB_KV4_REQS], start[LB_KV4_REQS], seq[LB_KV4_REQS], limit[KA_COLS], done;
         uint32_t requested, warp_sum[KA_WARPS];
     };
-    static_assert(sizeof(smem) <= LB_KV4_SMEM(D) && (LB_KV4_SMEM(D) + 1024) * LB_KV4_CTAS <= 228 * 1024, "shared memory");
+    static_assert(sizeof(smem) <= LB_KV4_SMEM && (LB_KV4_SMEM + 1024) * LB_KV4_CTAS <= 228 * 1024, "shared memory");
     const lb_kv4_attn_params& p;
     smem& s;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, g = lane >> 2, ft = lane & 3, G;
@@ -87,7 +93,7 @@ struct ka {
         if (t < p.b.n_reqs) q = kv4_get(p.b, t);
         const int len = q.n > 0 ? q.pos + q.n : 0;
         s.len[t] = len; s.n[t] = q.n; s.start[t] = q.start; s.seq[t] = q.seq;
-        uint32_t sum = q.n > 0 ? (uint32_t)((len + KA_TILE - 1) / KA_TILE) * p.b.HKV * sets(q.n) : 0u;
+        uint32_t sum = q.n > 0 ? (uint32_t)((len + TILE - 1) / TILE) * p.b.HKV * sets(q.n) : 0u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -115,7 +121,7 @@ struct ka {
         }
         ka_item it;
         it.r = lo;
-        it.tiles = (s.len[lo] + KA_TILE - 1) / KA_TILE;
+        it.tiles = (s.len[lo] + TILE - 1) / TILE;
         const int local = (int)(x - s.pre[lo]), item = local / it.tiles, z = sets(s.n[lo]);
         it.tile = local - item * it.tiles;
         it.kv = item / z;
@@ -130,14 +136,14 @@ struct ka {
         if (++it.kv < p.b.HKV) return;
         it.kv = 0;
         do ++it.r; while (it.r < p.b.n_reqs && s.n[it.r] <= 0);
-        it.tiles = it.r < p.b.n_reqs ? (s.len[it.r] + KA_TILE - 1) / KA_TILE : 0;
+        it.tiles = it.r < p.b.n_reqs ? (s.len[it.r] + TILE - 1) / TILE : 0;
     }
-    __device__ __forceinline__ int blocks(const ka_item& it) const { return min(8, (s.len[it.r] - it.tile * KA_TILE + 15) >> 4); }
+    __device__ __forceinline__ int blocks(const ka_item& it) const { return min(BLOCKS, (s.len[it.r] - it.tile * TILE + 15) >> 4); }
     // tile number i of this CTA
     __device__ __forceinline__ void copy(const ka_item& it, uint32_t i) const {
         const uint32_t bytes = (uint32_t)blocks(it) * BLK;
         mbar_arrive_expect_tx(&s.full[i % NS], bytes);
-        bulk_g2s_plain(s.ring[i % NS], p.b.cache + kv4_block(p.b, D, s.seq[it.r], it.kv, it.tile * KA_TILE), bytes, &s.full[i % NS]);
+        bulk_g2s_plain(s.ring[i % NS], p.b.cache + kv4_block(p.b, D, s.seq[it.r], it.kv, it.tile * TILE), bytes, &s.full[i % NS]);
     }
 
     // the queries of an item's columns: norm, rotation, 22 bits, as operands; a column per warp, a lane 8 features
@@ -211,15 +217,16 @@ struct ka {
     float m;            // reference of column g's scores, in log2 units
     float low[4];       // of this warp's rows, column g in two terms: sums of p lowest of groups 2 ft, 2 ft + 1; ft = 2: the sum of p
     float acc[8][2];    // of this warp's group and part, column g: features 8 (2 ft, 2 ft + 1) + j: of a for even j, of a + 16 b for odd ones
-    uint2 ref;          // fp16 bits of the scales that the groups' are taken against
+    uint32_t ref[S];    // fp16 bits, twice, of the scales that the groups' are taken against
+    uint32_t up[S];     // fp16 2^-1 over a reference's power of two, twice
 
-    __device__ __forceinline__ uint32_t ref_of(int q) const { return ((q & 2 ? ref.y : ref.x) >> (16 * (q & 1))) & 0xffffu; }
     __device__ __forceinline__ void begin() {
         m = -INFINITY;
         low[0] = low[1] = low[2] = low[3] = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = 0.f;
-        ref = make_uint2(0, 0);
+#pragma unroll
+        for (int q = 0; q < S; ++q) ref[q] = up[q] = 0u;
     }
 
     // (scale, lowest) of four rows, of those that are there
@@ -227,23 +234,36 @@ struct ka {
         return make_uint4(row0 < len ? v.x : 0u, row0 + 1 < len ? v.y : 0u, row0 + 2 < len ? v.z : 0u, row0 + 3 < len ? v.w : 0u);
     }
     static __device__ __forceinline__ uint32_t lowest_or_0(uint32_t pair) { return (pair & 0x7fff0000u) < 0x7c000000u ? pair : 0u; }
+    // a thread's scores of a block of 16 rows: rows row0 .. row0 + 3, column g; the values' scales of these rows as fp16 pairs
+    struct rows {
+        float sc[4];
+        uint32_t s01[S], s23[S];
+        uint2 hi, lo; // probabilities in two terms
+    };
+    // the largest scale of a group over these rows, in the halves of a word; a NaN has no say: columns before its row are not to notice it
+    static __device__ __forceinline__ uint32_t widest(uint32_t s01, uint32_t s23, bool edge) {
+        if (edge) {
+            s01 &= __vcmpltu2(s01, 0x7c007c00u);
+            s23 &= __vcmpltu2(s23, 0x7c007c00u);
+        }
+        return __vmaxu2(s01, s23);
+    }
 
-    // scores -> probabilities in two terms, p scale in shared memory
-    __device__ __forceinline__ void weigh(const float (&sc)[4], const uint4 (&scale)[(S + 1) / 2], float f, bool live, bool edge, int row0, uint2& hi, uint2& lo) {
+    // scores -> probabilities, p scale in shared memory
+    __device__ __forceinline__ void weigh(rows& r, int b, float f, bool edge, int row0) {
         const float less = KA_LIFT - (m == -INFINITY ? 0.f : m); // a column that has seen nothing yet
         float pr[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pr[i] = ka_exp2(fmaf(sc[i], f, less));
-        ka_split(pr[0], pr[1], hi.x, lo.x);
-        ka_split(pr[2], pr[3], hi.y, lo.y);
-        if (!live) return;
-        const int lim = edge ? s.limit[g] : 0x7fffffff;
+        for (int i = 0; i < 4; ++i) pr[i] = ka_exp2(fmaf(r.sc[i], f, less));
+        ka_split(pr[0], pr[1], r.hi.x, r.lo.x);
+        ka_split(pr[2], pr[3], r.hi.y, r.lo.y);
 #pragma unroll
         for (int q = 0; q < S; ++q) {
-            const float up = ka_pow2(-1 - ka_exponent(ref_of(q)));
-            const float2 s01 = ka_pair(q & 1 ? scale[q >> 1].z : scale[q >> 1].x), s23 = ka_pair(q & 1 ? scale[q >> 1].w : scale[q >> 1].y);
-            float w[4] = {pr[0] * (s01.x * up), pr[1] * (s01.y * up), pr[2] * (s23.x * up), pr[3] * (s23.y * up)};
+            const __half2 u = *reinterpret_cast<const __half2*>(&up[q]);
+            const float2 s01 = __half22float2(__hmul2(*reinterpret_cast<const __half2*>(&r.s01[q]), u)), s23 = __half22float2(__hmul2(*reinterpret_cast<const __half2*>(&r.s23[q]), u));
+            float w[4] = {pr[0] * s01.x, pr[1] * s01.y, pr[2] * s23.x, pr[3] * s23.y};
             if (edge) { // a NaN's group reaches the columns that see its row, and no other as 0 times NaN
+                const int lim = s.limit[g];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (row0 + i > lim) w[i] = 0.f;
@@ -251,134 +271,137 @@ struct ka {
             uint4 o;
             ka_split(w[0], w[1], o.x, o.y);
             ka_split(w[2], w[3], o.z, o.w);
-            s.p[q][warp][lane] = o;
+            s.p[q][b][lane] = o;
         }
     }
 
     // one tile; false: the wait for it gave up
     __device__ __forceinline__ bool tile(const ka_item& it, uint32_t i_tile, uint32_t tiles) {
-        const int slot = i_tile % NS, len = s.len[it.r], first_new = len - s.n[it.r];
-        const int nb = blocks(it), row0 = it.tile * KA_TILE + warp * 16 + 4 * ft; // this thread's rows: row0 .. row0 + 3
-        const bool edge = it.tile * KA_TILE + warp * 16 + 15 > first_new;           // rows that not every column sees, or that are not there
-        const unsigned char* blk = s.ring[slot] + warp * BLK;
+        const int slot = i_tile % NS, len = s.len[it.r], first_new = len - s.n[it.r], nb = blocks(it), base = it.tile * TILE + 16 * warp;
+        const bool edge = base + 128 * (BW - 1) + 15 > first_new; // rows that not every column sees, or that are not there
+        const unsigned char* ring = s.ring[slot];
         const float f = s.factor[g];
-        float sc[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        uint4 scale[(S + 1) / 2]; // values' scales of rows row0 .. row0 + 3 as fp16 pairs, two groups each
-        uint2 mx = make_uint2(0, 0);
+        rows r[BW];
+        bool landed = mbar_wait(&s.full[slot], (i_tile / NS) & 1), over = !landed;
+        if (warp < nb && landed) {
+            float a[BW][S][2][4];
+            uint2 w[BW][S][2];
+            uint32_t pair[BW][2];
 #pragma unroll
-        for (int q = 0; q < (S + 1) / 2; ++q) scale[q] = make_uint4(0, 0, 0, 0);
-        bool landed = mbar_wait(&s.full[slot], (i_tile / NS) & 1);
-        const bool live = warp < nb && landed;
-        if (live) {
-            float a[S][2][4];
-            uint2 w[S][2];
-            uint32_t pair[2];
-#pragma unroll
-            for (int q = 0; q < S; ++q)
+            for (int k = 0; k < BW; ++k) { // blocks that are not there hold what was there before them: their scores are masked
+                const unsigned char* blk = ring + (warp + 8 * k) * BLK;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    w[q][i] = *reinterpret_cast<const uint2*>(blk + ((i * S + q) * 32 + lane) * 8);
-                    a[q][i][0] = a[q][i][1] = a[q][i][2] = a[q][i][3] = 0.f;
+#pragma unroll
+                    for (int q = 0; q < S; ++q) w[k][q][i] = *reinterpret_cast<const uint2*>(blk + ((i * S + q) * 32 + lane) * 8);
+                    pair[k][i] = *reinterpret_cast<const uint32_t*>(blk + 16 * D + ((ft % S) * 16 + 4 * (g >> 1) + 2 * i + (g & 1)) * 4);
                 }
+            }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) pair[i] = *reinterpret_cast<const uint32_t*>(blk + 16 * D + ((ft % S) * 16 + 4 * (g >> 1) + 2 * i + (g & 1)) * 4);
-#pragma unroll
-            for (int st = 0; st < 4; ++st) // the groups are chains of their own
+            for (int st = 0; st < 4; ++st) // blocks and groups are chains of their own
 #pragma unroll
                 for (int q = 0; q < S; ++q) {
                     const uint4 qa = s.q[q * 4 + st][lane];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t v = st < 2 ? w[q][i].x : w[q][i].y, both = st & 1 ? __byte_perm(v, 0u, 0x4341) : v & 0x00ff00ffu;
-                        ka_mma(a[q][i], qa, (st & 1 ? both : v) & 0x000f000fu, both);
-                    }
+                    for (int k = 0; k < BW; ++k)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t v = st < 2 ? w[k][q][i].x : w[k][q][i].y, both = st & 1 ? __byte_perm(v, 0u, 0x4341) : v & 0x00ff00ffu, one = (st & 1 ? both : v) & 0x000f000fu;
+                            if (st == 0) ka_mma0(a[k][q][i], qa, one, both);
+                            else ka_mma(a[k][q][i], qa, one, both);
+                        }
                 }
-            {   // lowest sum(q)
-                const uint2 qs = s.qsum[lane];
+            const uint2 qs = s.qsum[lane];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-                    ka_mma(d, make_uint4(qs.x, qs.y, 0u, 0u), pair[i], 0u);
-                    sc[2 * i] = (d[0] + d[2]) * 3.814697265625e-06f; // 2^-18: the codes' 2^-24 over the sums' 2^-6
-                    sc[2 * i + 1] = (d[1] + d[3]) * 3.814697265625e-06f;
+            for (int k = 0; k < BW; ++k) {
+                const unsigned char* blk = ring + (warp + 8 * k) * BLK;
+                const int row0 = base + 128 * k + 4 * ft;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) { // lowest sum(q)
+                    float d[4];
+                    ka_mma0(d, make_uint4(qs.x, qs.y, 0u, 0u), pair[k][i], 0u);
+                    r[k].sc[2 * i] = (d[0] + d[2]) * 3.814697265625e-06f; // 2^-18: the codes' 2^-24 over the sums' 2^-6
+                    r[k].sc[2 * i + 1] = (d[1] + d[3]) * 3.814697265625e-06f;
                 }
-            }
 #pragma unroll
-            for (int q = 0; q < S; ++q) {
-                const uint4 pr = *reinterpret_cast<const uint4*>(blk + 16 * D + (q * 16 + 4 * ft) * 4);
-                sc[0] = fmaf(ka_pair(pr.x).x, a[q][0][0] + a[q][0][2], sc[0]);
-                sc[1] = fmaf(ka_pair(pr.y).x, a[q][0][1] + a[q][0][3], sc[1]);
-                sc[2] = fmaf(ka_pair(pr.z).x, a[q][1][0] + a[q][1][2], sc[2]);
-                sc[3] = fmaf(ka_pair(pr.w).x, a[q][1][1] + a[q][1][3], sc[3]);
-            }
-#pragma unroll
-            for (int q = 0; q < S; ++q) {
-                uint4 vr = *reinterpret_cast<const uint4*>(blk + 17 * D + (q * 16 + 4 * ft) * 4);
-                if (edge) vr = there(vr, row0, len);
-                uint32_t& s01 = q & 1 ? scale[q >> 1].z : scale[q >> 1].x;
-                uint32_t& s23 = q & 1 ? scale[q >> 1].w : scale[q >> 1].y;
-                s01 = __byte_perm(vr.x, vr.y, 0x5410);
-                s23 = __byte_perm(vr.z, vr.w, 0x5410);
-            }
-            // the largest scale of each group over these rows; scales are not negative
-            auto most = [&](uint4 v) {
-                if (edge) { // a NaN has no say: columns before its row are not to notice it
-                    v.x &= __vcmpltu2(v.x, 0x7c007c00u); v.y &= __vcmpltu2(v.y, 0x7c007c00u);
-                    v.z &= __vcmpltu2(v.z, 0x7c007c00u); v.w &= __vcmpltu2(v.w, 0x7c007c00u);
+                for (int q = 0; q < S; ++q) {
+                    const uint4 pr = *reinterpret_cast<const uint4*>(blk + 16 * D + (q * 16 + 4 * ft) * 4);
+                    r[k].sc[0] = fmaf(ka_pair(pr.x).x, a[k][q][0][0] + a[k][q][0][2], r[k].sc[0]);
+                    r[k].sc[1] = fmaf(ka_pair(pr.y).x, a[k][q][0][1] + a[k][q][0][3], r[k].sc[1]);
+                    r[k].sc[2] = fmaf(ka_pair(pr.z).x, a[k][q][1][0] + a[k][q][1][2], r[k].sc[2]);
+                    r[k].sc[3] = fmaf(ka_pair(pr.w).x, a[k][q][1][1] + a[k][q][1][3], r[k].sc[3]);
                 }
-                const uint32_t u = __vmaxu2(v.x, v.y), o = __vmaxu2(v.z, v.w);
-                return __vmaxu2(__byte_perm(u, o, 0x5410), __byte_perm(u, o, 0x7632));
-            };
-            mx.x = most(scale[0]);
-            if (S > 2) mx.y = most(scale[(S + 1) / 2 - 1]);
-            if (edge) {
-                const int lim = s.limit[g];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (row0 + i > lim) sc[i] = -INFINITY;
+                for (int q = 0; q < S; ++q) {
+                    uint4 vr = *reinterpret_cast<const uint4*>(blk + 17 * D + (q * 16 + 4 * ft) * 4);
+                    if (edge) vr = there(vr, row0, len);
+                    r[k].s01[q] = __byte_perm(vr.x, vr.y, 0x5410);
+                    r[k].s23[q] = __byte_perm(vr.z, vr.w, 0x5410);
+                    // does something pass its reference by more than there is room for?  A reference of 0 has none
+                    const uint32_t v = widest(r[k].s01[q], r[k].s23[q], edge);
+                    over |= v != __vminu2(v, ref[q] ? __vaddus2(ref[q], KA_WIDE) : 0u);
+                }
+                if (edge) {
+                    const int lim = s.limit[g];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (row0 + i > lim) r[k].sc[i] = -INFINITY;
+                }
+                over |= fmaf(fmaxf(fmaxf(r[k].sc[0], r[k].sc[1]), fmaxf(r[k].sc[2], r[k].sc[3])), f, -m) > KA_OVER;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < BW; ++k) {
+                r[k].sc[0] = r[k].sc[1] = r[k].sc[2] = r[k].sc[3] = -INFINITY;
+#pragma unroll
+                for (int q = 0; q < S; ++q) r[k].s01[q] = r[k].s23[q] = 0u;
             }
         }
-        const float best = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
-        // does something pass its reference by more than there is room for?  A reference of 0 has none
-        auto passes = [](uint32_t v, uint32_t r) { return v != __vminu2(v, __vaddus2(r, (KA_WIDE << 16 | KA_WIDE) & __vcmpgtu2(r, 0u))); };
-        const bool over = !landed || fmaf(best, f, -m) > KA_OVER || passes(mx.x, ref.x) || (S > 2 && passes(mx.y, ref.y));
         if (i_tile) landed = mbar_wait(&s.pfree, (i_tile - 1) & 1) && landed; // the tile before has been read out
-        uint2 hi, lo;
-        weigh(sc, scale, f, live, edge, row0, hi, lo);
+        if (warp < nb)
+#pragma unroll
+            for (int k = 0; k < BW; ++k) weigh(r[k], warp + 8 * k, f, edge, base + 128 * k + 4 * ft);
         if (__syncthreads_or(over || !landed)) {
             if (__syncthreads_or(!landed)) return false;
-            renew(sc, scale, mx, best, f, live, edge, row0, hi, lo);
+            renew(r, f, warp < nb, edge, base + 4 * ft);
         }
-        if (live) {
-            uint4 vr = *reinterpret_cast<const uint4*>(blk + 17 * D + ((g % S) * 16 + 4 * ft) * 4);
-            if (edge) { // where a column sees a NaN's row, p scale is NaN
-                vr = there(vr, row0, len);
-                vr.x = lowest_or_0(vr.x); vr.y = lowest_or_0(vr.y); vr.z = lowest_or_0(vr.z); vr.w = lowest_or_0(vr.w);
-            }
-            const uint32_t b0 = g == 4 ? 0x3c003c00u : __byte_perm(vr.x, vr.y, 0x7632), b1 = g == 4 ? 0x3c003c00u : __byte_perm(vr.z, vr.w, 0x7632);
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            ka_mma(d, make_uint4(hi.x, lo.x, hi.y, lo.y), b0, b1);
+        if (warp < nb) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) low[i] += d[i];
+            for (int k = 0; k < BW; ++k) {
+                uint4 vr = *reinterpret_cast<const uint4*>(ring + (warp + 8 * k) * BLK + 17 * D + ((g % S) * 16 + 4 * ft) * 4);
+                if (edge) { // where a column sees a NaN's row, p scale is NaN
+                    vr = there(vr, base + 128 * k + 4 * ft, len);
+                    vr.x = lowest_or_0(vr.x); vr.y = lowest_or_0(vr.y); vr.z = lowest_or_0(vr.z); vr.w = lowest_or_0(vr.w);
+                }
+                const uint32_t b0 = g == 4 ? 0x3c003c00u : __byte_perm(vr.x, vr.y, 0x7632), b1 = g == 4 ? 0x3c003c00u : __byte_perm(vr.z, vr.w, 0x7632);
+                float d[4];
+                ka_mma0(d, make_uint4(r[k].hi.x, r[k].lo.x, r[k].hi.y, r[k].lo.y), b0, b1);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) low[i] += d[i];
+            }
         }
-        {
-            const int group = warp % S, part = warp / S;
+        const int group = warp % S, part = warp / S;
+        if (part < nb) {
             float d[8][4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.f;
-#pragma unroll
-            for (int k = 0; k < S; ++k) {
-                const int b = part * S + k;
-                if (b >= nb) break;
-                const uint4 v = *reinterpret_cast<const uint4*>(s.ring[slot] + b * BLK + 8 * D + group * 512 + lane * 16);
+            for (int k = 0; k < 4; ++k) {
+                const int b = k * PARTS + part;
+                if (k && b >= nb) break;
+                const uint4 v = *reinterpret_cast<const uint4*>(ring + b * BLK + 8 * D + group * 512 + lane * 16);
                 const uint32_t a0 = __byte_perm(v.x, v.y, 0x5410), a1 = __byte_perm(v.x, v.y, 0x7632), c0 = __byte_perm(v.z, v.w, 0x5410), c1 = __byte_perm(v.z, v.w, 0x7632);
                 const uint4 pa = s.p[group][b][lane];
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const uint32_t y = j < 4 ? a0 : a1, z = j < 4 ? c0 : c1;
                     const uint32_t yb = j & 2 ? __byte_perm(y, 0u, 0x4341) : y & 0x00ff00ffu, zb = j & 2 ? __byte_perm(z, 0u, 0x4341) : z & 0x00ff00ffu;
-                    ka_mma(d[j], pa, (j & 2 ? yb : y) & 0x000f000fu, (j & 2 ? zb : z) & 0x000f000fu);
-                    ka_mma(d[j + 1], pa, yb, zb);
+                    const uint32_t y1 = (j & 2 ? yb : y) & 0x000f000fu, z1 = (j & 2 ? zb : z) & 0x000f000fu;
+                    if (k == 0) {
+                        ka_mma0(d[j], pa, y1, z1);
+                        ka_mma0(d[j + 1], pa, yb, zb);
+                    } else {
+                        ka_mma(d[j], pa, y1, z1);
+                        ka_mma(d[j + 1], pa, yb, zb);
+                    }
                 }
             }
 #pragma unroll
@@ -406,7 +429,20 @@ struct ka {
     }
 
     // new references: the exchange of maxima, and the probabilities again
-    __device__ __forceinline__ void renew(const float (&sc)[4], const uint4 (&scale)[(S + 1) / 2], uint2 mx, float best, float f, bool live, bool edge, int row0, uint2& hi, uint2& lo) {
+    __device__ __forceinline__ void renew(rows (&r)[BW], float f, bool live, bool edge, int row0) {
+        float best = -INFINITY;
+        uint2 mx = make_uint2(0u, 0u); // the groups' largest scales, 16 bits each
+#pragma unroll
+        for (int k = 0; k < BW; ++k) best = fmaxf(best, fmaxf(fmaxf(r[k].sc[0], r[k].sc[1]), fmaxf(r[k].sc[2], r[k].sc[3])));
+#pragma unroll
+        for (int q = 0; q < S; ++q) {
+            uint32_t v = 0u;
+#pragma unroll
+            for (int k = 0; k < BW; ++k) v = __vmaxu2(v, widest(r[k].s01[q], r[k].s23[q], edge));
+            v = max(v & 0xffffu, v >> 16) << (16 * (q & 1));
+            if (q & 2) mx.y |= v;
+            else mx.x |= v;
+        }
         best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
         best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
         if (ft == 0) s.max[g][warp] = best;
@@ -420,20 +456,31 @@ struct ka {
         const float4 a = *reinterpret_cast<const float4*>(s.max[g]), b = *reinterpret_cast<const float4*>(s.max[g] + 4);
         const float now = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))) * f, top = fmaxf(m, now);
         const float corr = top == -INFINITY ? 0.f : ka_exp2(m - top);
-        const uint32_t old = ref_of(warp % S);
         m = top;
+        mx = make_uint2(0u, 0u);
 #pragma unroll
         for (int w = 0; w < KA_WARPS; w += 2) {
             const uint4 v = *reinterpret_cast<const uint4*>(&s.scale[w]);
-            ref.x = __vmaxu2(ref.x, __vmaxu2(v.x, v.z));
-            if (S > 2) ref.y = __vmaxu2(ref.y, __vmaxu2(v.y, v.w));
+            mx.x = __vmaxu2(mx.x, __vmaxu2(v.x, v.z));
+            mx.y = __vmaxu2(mx.y, __vmaxu2(v.y, v.w));
         }
-        const float shrink = corr * ka_pow2(ka_exponent(old) - ka_exponent(ref_of(warp % S)));
+        float shrink = corr;
+#pragma unroll
+        for (int q = 0; q < S; ++q) {
+            const uint32_t v = __byte_perm(q & 2 ? mx.y : mx.x, 0u, q & 1 ? 0x3232 : 0x1010), old = ref[q];
+            ref[q] = __vmaxu2(old, v);
+            const int e = ka_exponent(ref[q] & 0xffffu);
+            if (q == warp % S) shrink = corr * ka_pow2(ka_exponent(old & 0xffffu) - e);
+            const __half2 u = __float2half2_rn(ka_pow2(-1 - e));
+            up[q] = *reinterpret_cast<const uint32_t*>(&u);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) low[i] *= corr;
 #pragma unroll
         for (int j = 0; j < 8; ++j) { acc[j][0] *= shrink; acc[j][1] *= shrink; }
-        weigh(sc, scale, f, live, edge, row0, hi, lo);
+        if (live)
+#pragma unroll
+            for (int k = 0; k < BW; ++k) weigh(r[k], warp + 8 * k, f, edge, row0 + 128 * k);
         __syncthreads();
     }
 
@@ -472,7 +519,11 @@ struct ka {
         if (2 * ft + 1 < S) s.part[warp][g][2 * ft + 1] = low[1] + low[3];
         if (ft == 2) s.part[warp][g][S] = low[0] + low[2];
         if (ft == 0 && warp == 0) s.m[g] = m;
-        const float even = ka_pow2(ka_exponent(ref_of(group)) + 25), odd = even * 0.0625f; // 2^24 over 2^(-1 - exponent)
+        int e = 0;
+#pragma unroll
+        for (int q = 0; q < S; ++q)
+            if (q == group) e = ka_exponent(ref[q] & 0xffffu);
+        const float even = ka_pow2(e + 25), odd = even * 0.0625f; // 2^24 over 2^(-1 - e)
         for (int turn = 0; turn < PARTS; ++turn) { // the parts of a tile one after the other
             __syncthreads();
             if (part == turn)
@@ -527,7 +578,8 @@ struct ka {
             if (t == 0) join->first = -1;
             return;
         }
-        const uint32_t x0 = (uint32_t)((uint64_t)blockIdx.x * total / ctas), x1 = (uint32_t)((uint64_t)(blockIdx.x + 1) * total / ctas);
+        const uint32_t share = total / ctas, more = total - share * ctas; // the first `more` CTAs have one tile more
+        const uint32_t x0 = blockIdx.x * share + min(blockIdx.x, more), x1 = x0 + share + (blockIdx.x < more);
         ka_item it = place(x0);
         if (t == 0) {
             ka_item a = it;
@@ -563,9 +615,9 @@ struct ka {
             lb_kv4_join j;
             j.first = -1;
             const uint32_t begin = x0 - (uint32_t)at.tile, end = begin + (uint32_t)at.tiles;
-            if (at.tile > 0 && begin >= (uint32_t)((uint64_t)(blockIdx.x - 1) * total / ctas)) {
+            if (at.tile > 0 && begin >= x0 - share - (blockIdx.x - 1 < more)) {
                 j.first = (int)blockIdx.x - 1;
-                j.last = (int)(((uint64_t)end * ctas - 1) / total); // the CTA of tile end - 1: the last c with c total / ctas <= end - 1
+                j.last = (int)(end - 1 < more * (share + 1) ? (end - 1) / (share + 1) : more + (end - 1 - more * (share + 1)) / share); // the CTA of tile end - 1
                 j.row0 = s.start[at.r];
                 j.kv = at.kv;
                 j.col0 = at.z * KA_COLS;
@@ -586,97 +638,115 @@ KA_KERNEL(64)
 KA_KERNEL(128)
 KA_KERNEL(256)
 
-// Joins the records of the items that were cut.  Every CTA lists the joins; (join, column) pairs are dealt to the CTAs.  Records are added in the order of the rows, in runs
-// of neighbours side by side, so results are the same from run to run.
-#define KM_THREADS 1024
-#define KM_JOINS 512 /* CTAs of the attention kernel at most */
+// Joins the records of the items that were cut.  Every CTA counts the joins' columns; (join, column) pairs are dealt to groups of D / 4 threads, or to whole CTAs in which such
+// groups take runs of neighbouring records where there are few.  Records are added in the order of the rows, so results are the same from run to run.
+#define KM_THREADS 256
 template <int D>
 __device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int ctas) {
-    constexpr int SUB = KM_THREADS / D; // runs of records side by side
-    __shared__ float red[3][KM_THREADS];
-    __shared__ int s_join[KM_JOINS], s_before[KM_JOINS + 1], s_warp[KM_JOINS / 32][2];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    constexpr int W = D / 4, SUB = KM_THREADS / W; // threads of a group, groups
+    __shared__ float4 red[KM_THREADS];
+    __shared__ float red_m[SUB], red_l[SUB];
+    __shared__ int pre[LB_KV4_MAX_CTAS + 1], s_warp[KM_THREADS / 32];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, sub = t / W, f = t % W * 4, G = p.HQ / p.b.HKV;
     pdl_wait();
-    int cols = 0;
-    if (t < ctas && p.joins[t].first >= 0) cols = p.joins[t].cols;
-    const uint32_t on = __ballot_sync(0xffffffffu, cols > 0);
-    int sum = cols;
+    int base = 0;
+    if (t == 0) pre[0] = 0;
+    for (int c0 = 0; c0 < ctas; c0 += KM_THREADS) { // columns before every join
+        int sum = 0;
+        if (c0 + t < ctas && p.joins[c0 + t].first >= 0) sum = p.joins[c0 + t].cols;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-    }
-    if (lane == 31 && warp < KM_JOINS / 32) {
-        s_warp[warp][0] = __popc(on);
-        s_warp[warp][1] = sum;
-    }
-    __syncthreads();
-    int joins = 0, pairs = 0, at = __popc(on & ((1u << lane) - 1u)), before = sum - cols;
-#pragma unroll
-    for (int w = 0; w < KM_JOINS / 32; ++w) {
-        if (w == warp) { at += joins; before += pairs; }
-        joins += s_warp[w][0];
-        pairs += s_warp[w][1];
-    }
-    if (cols > 0) {
-        s_join[at] = t;
-        s_before[at] = before;
-    }
-    __syncthreads();
-    const int f = t % D, sub = t / D, G = p.HQ / p.b.HKV;
-    int k = 0;
-    for (int pair = blockIdx.x; pair < pairs; pair += gridDim.x) {
-        while (k + 1 < joins && s_before[k + 1] <= pair) ++k;
-        const lb_kv4_join j = p.joins[s_join[k]];
-        const int c = pair - s_before[k], per = (j.last - j.first + SUB) / SUB; // records of a run
-        float M = -INFINITY, L = 0.f, A = 0.f;
-        const int b0 = j.first + sub * per, b1 = min(j.last + 1, b0 + per);
-        for (int b = b0; b < b1; b += 8) {
-            float mv[8], lv[8], av[8], mx = M;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool there = b + i < b1;
-                const float* rec = p.records + (((size_t)(there ? b + i : b) * 2 + (b + i == j.first ? 1 : 0)) * KA_COLS + c) * LB_KV4_REC(D);
-                mv[i] = there ? __ldcg(rec + D) : -INFINITY;
-                lv[i] = there ? __ldcg(rec + D + 1) : 0.f;
-                av[i] = there ? __ldcg(rec + f) : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, mv[i]);
-            const float use = mx == -INFINITY ? 0.f : mx, w = ka_exp2(M - use);
-            L *= w;
-            A *= w;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = ka_exp2(mv[i] - use);
-                L = fmaf(lv[i], v, L);
-                A = fmaf(av[i], v, A);
-            }
-            M = mx;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
         }
-        red[0][t] = M;
-        red[1][t] = L;
-        red[2][t] = A;
+        if (lane == 31) s_warp[warp] = sum;
         __syncthreads();
-        if (sub == 0) {
-            float mx = M;
+        int all = 0;
 #pragma unroll
-            for (int q = 1; q < SUB; ++q) mx = fmaxf(mx, red[0][q * D + f]);
-            const float use = mx == -INFINITY ? 0.f : mx;
-            L = A = 0.f;
-#pragma unroll
-            for (int q = 0; q < SUB; ++q) {
-                const float v = ka_exp2(red[0][q * D + f] - use);
-                L = fmaf(red[1][q * D + f], v, L);
-                A = fmaf(red[2][q * D + f], v, A);
+        for (int w = 0; w < KM_THREADS / 32; ++w) {
+            if (w < warp) sum += s_warp[w];
+            all += s_warp[w];
+        }
+        if (c0 + t < ctas) pre[c0 + t + 1] = base + sum;
+        base += all;
+        __syncthreads();
+    }
+    const int pairs = base;
+    const bool few = pairs <= (int)gridDim.x; // a CTA for each
+    for (int first = few ? (int)blockIdx.x : (int)blockIdx.x * SUB; first < pairs; first += few ? (int)gridDim.x : (int)gridDim.x * SUB) {
+        const int pair = few ? first : first + sub;
+        float M = -INFINITY, L = 0.f;
+        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+        lb_kv4_join j;
+        int c = 0;
+        if (pair < pairs) {
+            int lo = 0, hi = ctas - 1; // the last join with pre <= pair
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (pre[mid] <= pair) lo = mid;
+                else hi = mid - 1;
             }
+            j = p.joins[lo];
+            c = pair - pre[lo];
+            const int n = j.last - j.first + 1, per = few ? (n + SUB - 1) / SUB : n, b0 = j.first + (few ? sub * per : 0), b1 = min(j.last + 1, b0 + per);
+            for (int b = b0; b < b1; b += 8) {
+                float mv[8], lv[8], mx = M;
+                float4 av[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const bool on = b + i < b1;
+                    const float* rec = p.records + (((size_t)(on ? b + i : b) * 2 + (b + i == j.first ? 1 : 0)) * KA_COLS + c) * LB_KV4_REC(D);
+                    mv[i] = on ? __ldcg(rec + D) : -INFINITY;
+                    lv[i] = on ? __ldcg(rec + D + 1) : 0.f;
+                    av[i] = on ? __ldcg(reinterpret_cast<const float4*>(rec + f)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, mv[i]);
+                const float use = mx == -INFINITY ? 0.f : mx, w = ka_exp2(M - use);
+                L *= w;
+                A.x *= w; A.y *= w; A.z *= w; A.w *= w;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = ka_exp2(mv[i] - use);
+                    L = fmaf(lv[i], v, L);
+                    A.x = fmaf(av[i].x, v, A.x); A.y = fmaf(av[i].y, v, A.y); A.z = fmaf(av[i].z, v, A.z); A.w = fmaf(av[i].w, v, A.w);
+                }
+                M = mx;
+            }
+        }
+        if (few) {
+            red[t] = A;
+            if (t % W == 0) { red_m[sub] = M; red_l[sub] = L; }
+            __syncthreads();
+            if (sub == 0) {
+                float mx = M;
+#pragma unroll
+                for (int q = 1; q < SUB; ++q) mx = fmaxf(mx, red_m[q]);
+                const float use = mx == -INFINITY ? 0.f : mx;
+                L = 0.f;
+                A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int q = 0; q < SUB; ++q) {
+                    const float v = ka_exp2(red_m[q] - use);
+                    const float4 x = red[q * W + t];
+                    L = fmaf(red_l[q], v, L);
+                    A.x = fmaf(x.x, v, A.x); A.y = fmaf(x.y, v, A.y); A.z = fmaf(x.z, v, A.z); A.w = fmaf(x.w, v, A.w);
+                }
+            }
+            __syncthreads();
+        }
+        if (pair < pairs && (!few || sub == 0)) {
             const int col = j.col0 + c, i = col / G, h = j.kv * G + col - i * G;
             const size_t row = (size_t)(j.row0 + i);
-            float v = A / L;
-            if (p.gate) v *= sigmoidf_dev(kv4_load1(p.gate, row * (size_t)p.row_stride + (size_t)h * (size_t)p.head_stride + f, p.type));
-            p.out[(row * p.HQ + h) * D + f] = __half_as_ushort(__float2half_rn(v));
+            const float inv = 1.f / L;
+            float v[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
+            uint16_t* d = p.out + (row * p.HQ + h) * D + f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (p.gate) v[k] *= sigmoidf_dev(kv4_load1(p.gate, row * (size_t)p.row_stride + (size_t)h * (size_t)p.head_stride + f + k, p.type));
+                d[k] = __half_as_ushort(__float2half_rn(v[k]));
+            }
         }
-        __syncthreads();
     }
 }
 extern "C" __global__ void __launch_bounds__(KM_THREADS) kv4_merge_64(const __grid_constant__ lb_kv4_attn_params p, int ctas) { kv4_merge_body<64>(p, ctas); }

@@ -598,12 +598,13 @@ typedef struct {
     int32_t out_wide;       /* out is 16-byte aligned */
     double freq[128];
 } lb_kv4_attn_params;
-/* The attention kernel: columns taken at a time, rows of a tile, CTAs per SM, ring stages.  Shared memory: the ring, probabilities, queries, the rest */
+/* The attention kernel: columns taken at a time, rows of a tile (36 KB), CTAs per SM and at most, ring stages.  Shared memory: the ring, probabilities, queries, the rest */
 #define LB_KV4_COLS 8
-#define LB_KV4_TILE 128
+#define LB_KV4_TILE(D) (32768 / (D))
 #define LB_KV4_CTAS 2
-#define LB_KV4_STAGES(D) ((D) == 256 ? 2 : (D) == 128 ? 4 : 6)
-#define LB_KV4_SMEM(D) (LB_KV4_STAGES(D) * 8 * LB_KV4_BLOCK(D) + (D) * 96 + 8 * 1024)
+#define LB_KV4_MAX_CTAS 1024
+#define LB_KV4_STAGES 2
+#define LB_KV4_SMEM (LB_KV4_STAGES * 36864 + 16384 + 8192 + 8 * 1024)
 
 /* ---- drafted tokens against the target's probabilities (verify.cu) -------------------------------------------- */
 #define LB_VD_REQS 256
