@@ -38,10 +38,11 @@ static int rotation(lb_ctx* c, const char* call, int dim, int rot_dims, float th
     return LB_OK;
 }
 
-/* units of a CTA of 256 threads (D / 8 threads each) make this many rows */
-static unsigned rows_grid(int rows, int kv_heads, int dim) {
-    const int units = 256 / (dim / 8), per_row = 2 * kv_heads, r = per_row < units ? units / per_row : 1;
-    return (unsigned)(((int64_t)rows + r - 1) / r);
+/* Rows of a CTA: as many as its 256 threads take at a time (D / 8 threads for a key or value vector), more where that would make more than four CTAs an SM */
+static unsigned rows_grid(const lb_ctx* c, lb_kv4_rows_params* p) {
+    const int units = 256 / (p->D / 8), per_row = 2 * p->b.HKV, fill = per_row < units ? units / per_row : 1, even = (p->b.rows + 4 * c->sm_count - 1) / (4 * c->sm_count);
+    p->chunk = even > fill ? even : fill;
+    return (unsigned)((p->b.rows + p->chunk - 1) / p->chunk);
 }
 
 static int by_dim(int dim, int k64, int k128, int k256) { return dim == 64 ? k64 : dim == 128 ? k128 : k256; }
@@ -60,7 +61,7 @@ LB_API int lb_kv4_append(lb_ctx* c, const lb_kv4_cache* cache, const lb_kv4_batc
     p.stride = stride; p.D = cache->dim; p.type = type; p.rot_dims = rot_dims; p.eps = (double)eps;
     p.wide = ((k | v | (uint64_t)stride * (uint64_t)size_of(type)) & 15) == 0;
     void* params[] = {&p};
-    return lb_launch(c, by_dim(cache->dim, LBK_kv4_append_64, LBK_kv4_append_128, LBK_kv4_append_256), rows_grid(batch->rows, cache->kv_heads, cache->dim), 1, 1, 256, 0, params, 1);
+    return lb_launch(c, by_dim(cache->dim, LBK_kv4_append_64, LBK_kv4_append_128, LBK_kv4_append_256), rows_grid(c, &p), 1, 1, 256, 0, params, 1);
 }
 
 LB_API int lb_kv4_read(lb_ctx* c, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t k_out, uint64_t v_out, int type) {
@@ -72,7 +73,7 @@ LB_API int lb_kv4_read(lb_ctx* c, const lb_kv4_cache* cache, const lb_kv4_batch*
     p.D = cache->dim; p.type = type;
     p.wide = ((k_out | v_out) & 15) == 0;
     void* params[] = {&p};
-    return lb_launch(c, by_dim(cache->dim, LBK_kv4_read_64, LBK_kv4_read_128, LBK_kv4_read_256), rows_grid(batch->rows, cache->kv_heads, cache->dim), 1, 1, 256, 0, params, 1);
+    return lb_launch(c, by_dim(cache->dim, LBK_kv4_read_64, LBK_kv4_read_128, LBK_kv4_read_256), rows_grid(c, &p), 1, 1, 256, 0, params, 1);
 }
 
 LB_API int lb_kv4_attention(lb_ctx* c, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t q, uint64_t gate, int64_t row_stride, int64_t head_stride, int type,

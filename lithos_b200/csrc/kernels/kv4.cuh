@@ -37,7 +37,7 @@ __device__ __forceinline__ kv4_request kv4_get(const lb_kv4_view& b, int r) {
     else if (q.pos < 0 || q.pos > b.max_ctx - q.n) bad = LB_DEV_POS_RANGE;
     if (bad) {
         atomicExch(b.status, bad);
-        q.n = 0;
+        q.n = q.start = 0;
     }
     return q;
 }

@@ -575,6 +575,7 @@ typedef struct {
     const uint16_t* norm_w; /* bf16 [D] or NULL */
     int64_t stride;
     int32_t D, type, rot_dims, wide; /* wide: rows may be read 16 bytes at a time */
+    int32_t chunk, pad_;    /* rows of a CTA */
     double eps;
     double freq[128];
 } lb_kv4_rows_params;
