@@ -44,6 +44,12 @@ __device__ __forceinline__ float ka_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// has the phase completed?  (no waiting)
+__device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
 // fp16 pairs of (x, y) and of what the rounding left
 __device__ __forceinline__ void ka_split(float x, float y, uint32_t& hi, uint32_t& lo) {
     hi = ka_pack(x, y);
@@ -75,8 +81,8 @@ struct ka {
         uint64_t full[NS], pfree;
         ka_item ahead;                  // the last tile that was requested
         uint32_t pre[LB_KV4_REQS + 1];  // tiles before request r
-        int len[LB_KV4_REQS], n[LB_KV4_REQS], start[LB_KV4_REQS], seq[LB_KV4_REQS], limit[KA_COLS], done;
-        uint32_t requested, warp_sum[KA_WARPS];
+        int len[LB_KV4_REQS], n[LB_KV4_REQS], start[LB_KV4_REQS], seq[LB_KV4_REQS], limit[KA_COLS];
+        uint32_t requested, warp_sum[KA_WARPS]; // requested: tiles of this CTA
     };
     static_assert(sizeof(smem) <= LB_KV4_SMEM && (LB_KV4_SMEM + 1024) * LB_KV4_CTAS <= 228 * 1024, "shared memory");
     const lb_kv4_attn_params& p;
@@ -219,8 +225,12 @@ struct ka {
     float acc[8][2];    // of this warp's group and part, column g: features 8 (2 ft, 2 ft + 1) + j: of a for even j, of a + 16 b for odd ones
     uint32_t ref[S];    // fp16 bits, twice, of the scales that the groups' are taken against
     uint32_t up[S];     // fp16 2^-1 over a reference's power of two, twice
+    float f;            // of column g's scores
+    int len, first_new; // rows of the item, the first of its new ones
 
-    __device__ __forceinline__ void begin() {
+    __device__ __forceinline__ void begin(const ka_item& it) {
+        len = s.len[it.r];
+        first_new = len - s.n[it.r];
         m = -INFINITY;
         low[0] = low[1] = low[2] = low[3] = 0.f;
 #pragma unroll
@@ -250,7 +260,7 @@ struct ka {
     }
 
     // scores -> probabilities, p scale in shared memory
-    __device__ __forceinline__ void weigh(rows& r, int b, float f, bool edge, int row0) {
+    __device__ __forceinline__ void weigh(rows& r, int b, bool edge, int row0) {
         const float less = KA_LIFT - (m == -INFINITY ? 0.f : m); // a column that has seen nothing yet
         float pr[4];
 #pragma unroll
@@ -277,10 +287,9 @@ struct ka {
 
     // one tile; false: the wait for it gave up
     __device__ __forceinline__ bool tile(const ka_item& it, uint32_t i_tile, uint32_t tiles) {
-        const int slot = i_tile % NS, len = s.len[it.r], first_new = len - s.n[it.r], nb = blocks(it), base = it.tile * TILE + 16 * warp;
+        const int slot = i_tile % NS, nb = min(BLOCKS, (len - it.tile * TILE + 15) >> 4), base = it.tile * TILE + 16 * warp;
         const bool edge = base + 128 * (BW - 1) + 15 > first_new; // rows that not every column sees, or that are not there
         const unsigned char* ring = s.ring[slot];
-        const float f = s.factor[g];
         rows r[BW];
         bool landed = mbar_wait(&s.full[slot], (i_tile / NS) & 1), over = !landed;
         if (warp < nb && landed) {
@@ -355,30 +364,27 @@ struct ka {
                 r[k].sc[0] = r[k].sc[1] = r[k].sc[2] = r[k].sc[3] = -INFINITY;
 #pragma unroll
                 for (int q = 0; q < S; ++q) r[k].s01[q] = r[k].s23[q] = 0u;
+                r[k].hi = r[k].lo = make_uint2(0u, 0u);
             }
         }
         if (i_tile) landed = mbar_wait(&s.pfree, (i_tile - 1) & 1) && landed; // the tile before has been read out
         if (warp < nb)
 #pragma unroll
-            for (int k = 0; k < BW; ++k) weigh(r[k], warp + 8 * k, f, edge, base + 128 * k + 4 * ft);
+            for (int k = 0; k < BW; ++k) weigh(r[k], warp + 8 * k, edge, base + 128 * k + 4 * ft);
         if (__syncthreads_or(over || !landed)) {
             if (__syncthreads_or(!landed)) return false;
-            renew(r, f, warp < nb, edge, base + 4 * ft);
+            renew(r, warp < nb, edge, base + 4 * ft);
         }
-        if (warp < nb) {
+        uint32_t lv[BW][2]; // p lowest and the sum of p: lowest values as an operand, ones in its fifth column
 #pragma unroll
-            for (int k = 0; k < BW; ++k) {
-                uint4 vr = *reinterpret_cast<const uint4*>(ring + (warp + 8 * k) * BLK + 17 * D + ((g % S) * 16 + 4 * ft) * 4);
-                if (edge) { // where a column sees a NaN's row, p scale is NaN
-                    vr = there(vr, base + 128 * k + 4 * ft, len);
-                    vr.x = lowest_or_0(vr.x); vr.y = lowest_or_0(vr.y); vr.z = lowest_or_0(vr.z); vr.w = lowest_or_0(vr.w);
-                }
-                const uint32_t b0 = g == 4 ? 0x3c003c00u : __byte_perm(vr.x, vr.y, 0x7632), b1 = g == 4 ? 0x3c003c00u : __byte_perm(vr.z, vr.w, 0x7632);
-                float d[4];
-                ka_mma0(d, make_uint4(r[k].hi.x, r[k].lo.x, r[k].hi.y, r[k].lo.y), b0, b1);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) low[i] += d[i];
+        for (int k = 0; k < BW; ++k) {
+            uint4 vr = *reinterpret_cast<const uint4*>(ring + (warp + 8 * k) * BLK + 17 * D + ((g % S) * 16 + 4 * ft) * 4);
+            if (edge) { // blocks that are not there, too; where a column sees a NaN's row, p scale is NaN
+                vr = there(vr, base + 128 * k + 4 * ft, len);
+                vr.x = lowest_or_0(vr.x); vr.y = lowest_or_0(vr.y); vr.z = lowest_or_0(vr.z); vr.w = lowest_or_0(vr.w);
             }
+            lv[k][0] = g == 4 ? 0x3c003c00u : __byte_perm(vr.x, vr.y, 0x7632);
+            lv[k][1] = g == 4 ? 0x3c003c00u : __byte_perm(vr.z, vr.w, 0x7632);
         }
         const int group = warp % S, part = warp / S;
         if (part < nb) {
@@ -410,26 +416,28 @@ struct ka {
                 acc[j][1] += d[j][1] + d[j][3];
             }
         }
+#pragma unroll
+        for (int k = 0; k < BW; ++k) {
+            float d[4];
+            ka_mma0(d, make_uint4(r[k].hi.x, r[k].lo.x, r[k].hi.y, r[k].lo.y), lv[k][0], lv[k][1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) low[i] += d[i];
+        }
         __syncwarp();
-        if (lane == 0) { // the last warp to be done requests what comes to this place next
+        if (lane == 0) { // whoever finds that all warps are done, the last one at least, requests what comes to this place next
             mbar_arrive(&s.pfree);
-            __threadfence_block();
-            if (atomicAdd(&s.done, 1) == KA_WARPS - 1) {
-                s.done = 0;
-                __threadfence_block();
-                if (s.requested < tiles) {
-                    ka_item a = s.ahead;
-                    next(a);
-                    s.ahead = a;
-                    copy(a, s.requested++);
-                }
+            if (i_tile + NS < tiles && mbar_try(&s.pfree, i_tile & 1) && atomicExch(&s.requested, i_tile + NS + 1) != i_tile + NS + 1) {
+                ka_item a = s.ahead;
+                next(a);
+                s.ahead = a;
+                copy(a, i_tile + NS);
             }
         }
         return true;
     }
 
     // new references: the exchange of maxima, and the probabilities again
-    __device__ __forceinline__ void renew(rows (&r)[BW], float f, bool live, bool edge, int row0) {
+    __device__ __forceinline__ void renew(rows (&r)[BW], bool live, bool edge, int row0) {
         float best = -INFINITY;
         uint2 mx = make_uint2(0u, 0u); // the groups' largest scales, 16 bits each
 #pragma unroll
@@ -480,7 +488,7 @@ struct ka {
         for (int j = 0; j < 8; ++j) { acc[j][0] *= shrink; acc[j][1] *= shrink; }
         if (live)
 #pragma unroll
-            for (int k = 0; k < BW; ++k) weigh(r[k], warp + 8 * k, f, edge, row0 + 128 * k);
+            for (int k = 0; k < BW; ++k) weigh(r[k], warp + 8 * k, edge, row0 + 128 * k);
         __syncthreads();
     }
 
@@ -568,7 +576,6 @@ struct ka {
             for (int i = 0; i < NS; ++i) mbar_init(&s.full[i], 1);
             mbar_init(&s.pfree, KA_WARPS);
             mbar_fence_init();
-            s.done = 0;
         }
         pdl_wait();
         const uint32_t total = read_batch(); // its barriers also show the mbarriers to everybody
@@ -596,8 +603,9 @@ struct ka {
             if (x == x0 || it.tile == 0) {
                 first = it.tile == 0;
                 queries(it);
-                begin();
+                begin(it);
                 __syncthreads();
+                f = s.factor[g];
             }
             if (!tile(it, x - x0, x1 - x0)) { // a copy never landed: say so, let the others land, leave
                 if (t == 0) {
