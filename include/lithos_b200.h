@@ -296,7 +296,7 @@ typedef struct {
 typedef struct {
     uint64_t seqs, pos, starts; /* i32 [n_reqs], [n_reqs], [n_reqs + 1] */
     int32_t n_reqs;             /* 1 .. LB_KV4_MAX_REQS */
-    int32_t rows;               /* token rows that the call's tensors have */
+    int32_t rows;               /* token rows that the call's tensors have, up to 2^24 */
 } lb_kv4_batch;
 size_t lb_kv4_bytes(int n_seqs, int max_ctx, int kv_heads, int dim); /* 0: not a shape of these calls */
 /* New rows into the cache.  k, v: element type `type`, heads next to each other, token rows `stride` elements apart (0: kv_heads * dim).  Keys are normalised
@@ -309,7 +309,8 @@ int lb_kv4_read(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batc
 /* Attention of the batch's new tokens, whose rows are in the cache: token i of request r sees rows 0 .. pos[r] + i.
  * q and gate (0: none): element type `type`, head h of token row j at j * row_stride + h * head_stride elements (row_stride 0: n_heads * head_stride, head_stride 0: dim); q is
  * normalised per head (q_norm_w; 0: not) and rotated like the keys, then rounded to fp16; the result is multiplied by sigmoid(gate).  n_heads: 1 to 16 times
- * kv_heads.  max_new: the most tokens a request of the batch has, 1 .. LB_KV4_MAX_NEW.  out fp16 [rows, n_heads, dim], what lb_gemm_int4 takes. */
+ * kv_heads.  max_new: the most tokens a request of the batch has, 1 .. LB_KV4_MAX_NEW.  out fp16 [rows, n_heads, dim], what lb_gemm_int4 takes; it
+ * overlaps none of the inputs. */
 int lb_kv4_attention(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t q, uint64_t gate, int64_t row_stride, int64_t head_stride, int type,
                      uint64_t q_norm_w, uint64_t out_f16, int n_heads, int max_new, int rot_dims, float rope_theta, float eps);
 /* Drafted tokens against the target's probabilities, for speculative decoding (with lb_model_checkpoint / lb_model_rollback for a model's recurrent state, or over the

@@ -18,8 +18,8 @@ static int view(lb_ctx* c, const char* call, const lb_kv4_cache* k, const lb_kv4
     if (!shape_ok(k->n_seqs, k->max_ctx, k->kv_heads, k->dim) || k->data % 16)
         return lb_fail(c, LB_ERR_INVALID, "%s: cache of %d x %d rows, %d heads of %d (max_ctx %% 16, up to 2^20; 1..32 heads of 64, 128 or 256; 16-byte aligned)", call, k->n_seqs,
                        k->max_ctx, k->kv_heads, k->dim);
-    if (b->n_reqs < 1 || b->n_reqs > LB_KV4_REQS || b->rows < 1 || (!b->starts && b->rows != b->n_reqs))
-        return lb_fail(c, LB_ERR_INVALID, "%s: %d requests, %d token rows (1..%d requests; without starts one row each)", call, b->n_reqs, b->rows, LB_KV4_REQS);
+    if (b->n_reqs < 1 || b->n_reqs > LB_KV4_REQS || b->rows < 1 || b->rows > LB_KV4_ROWS || (!b->starts && b->rows != b->n_reqs))
+        return lb_fail(c, LB_ERR_INVALID, "%s: %d requests, %d token rows (1..%d requests, 1..2^24 rows; without starts one row each)", call, b->n_reqs, b->rows, LB_KV4_REQS);
     if (((b->pos | b->seqs | b->starts) & 3) != 0) return lb_fail(c, LB_ERR_INVALID, "%s: arrays of 32-bit numbers must be 4-byte aligned", call);
     memset(v, 0, sizeof *v);
     v->cache = (unsigned char*)k->data;
@@ -95,7 +95,7 @@ LB_API int lb_kv4_attention(lb_ctx* c, const lb_kv4_cache* cache, const lb_kv4_b
     p.records = (float*)c->kv4_records; p.joins = (lb_kv4_join*)c->kv4_joins;
     p.row_stride = row_stride; p.head_stride = head_stride;
     p.HQ = n_heads; p.type = type; p.rot_dims = rot_dims; p.eps = eps;
-    p.wide = ((q | (uint64_t)row_stride * (uint64_t)size_of(type) | (uint64_t)head_stride * (uint64_t)size_of(type)) & 15) == 0;
+    p.wide = ((q | gate | (uint64_t)row_stride * (uint64_t)size_of(type) | (uint64_t)head_stride * (uint64_t)size_of(type)) & 15) == 0;
     p.out_wide = out % 16 == 0;
     /* no more CTAs than tiles that a full cache would have */
     const int64_t most = (int64_t)batch->n_reqs * HKV * sets * ((cache->max_ctx + LB_KV4_TILE(D) - 1) / LB_KV4_TILE(D));

@@ -56,6 +56,12 @@ __device__ __forceinline__ void ka_split(float x, float y, uint32_t& hi, uint32_
     const float2 h = ka_pair(hi);
     lo = ka_pack(x - h.x, y - h.y);
 }
+__device__ __forceinline__ void ka_scale(uint32_t hi, uint32_t lo, uint32_t scale, uint32_t up, uint32_t& first, uint32_t& rest) {
+    const __half2 h = *reinterpret_cast<const __half2*>(&hi), l = *reinterpret_cast<const __half2*>(&lo);
+    const __half2 s = __hmul2(*reinterpret_cast<const __half2*>(&scale), *reinterpret_cast<const __half2*>(&up)), f = __hmul2(h, s), r = __hfma2(l, s, __hfma2(h, s, __hneg2(f)));
+    first = *reinterpret_cast<const uint32_t*>(&f);
+    rest = *reinterpret_cast<const uint32_t*>(&r);
+}
 // exponent of a scale from its fp16 bits: below 2^(e + 1); scales below 2^-14 count as that
 __device__ __forceinline__ int ka_exponent(uint32_t bits) { return max((int)(bits >> 10), 1) - 15; }
 
@@ -77,6 +83,7 @@ struct ka {
         float part[KA_WARPS][KA_COLS][S + 1];
         alignas(16) float max[KA_COLS][KA_WARPS];
         alignas(16) uint2 scale[KA_WARPS];
+        double freq[D / 2];
         float factor[KA_COLS], m[KA_COLS], l[KA_COLS], low[KA_COLS][S];
         uint64_t full[NS], pfree;
         ka_item ahead;                  // the last tile that was requested
@@ -160,17 +167,23 @@ struct ka {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = 0.f;
         if (mine) kv4_load8(p.q, (size_t)(s.start[it.r] + i) * (size_t)p.row_stride + (size_t)h * (size_t)p.head_stride + lane * 8, p.type, p.wide, x);
-        float cs[4], sn[4];
+        // while the queries are on their way: angles in 64 bits, reduced to a turn, sine and cosine of at most pi in 32; a pair of features per lane, handed to the lane that has it
+        float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
+        if (on)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) { // while the queries are on their way: the angle in 64 bits, reduced to a turn; sine and cosine of at most pi in 32
-            cs[j] = 1.f;
-            sn[j] = 0.f;
-            const int f = lane * 4 + j;
-            if (mine && 2 * f < p.rot_dims) {
-                const double a = (double)(pos + i) * p.freq[f];
-                sincosf((float)fma(-rint(a * 0.15915494309189535), 6.283185307179586, a), &sn[j], &cs[j]);
+            for (int k = 0; k < D / 64; ++k) {
+                if (64 * k >= p.rot_dims) break;
+                float c1 = 1.f, s1 = 0.f;
+                if (2 * (32 * k + lane) < p.rot_dims) {
+                    const double a = (double)(pos + i) * s.freq[32 * k + lane];
+                    sincosf((float)fma(-rint(a * 0.15915494309189535), 6.283185307179586, a), &s1, &c1);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { // pairs 4 lane + j: of the eight lanes from 8 k on
+                    const float c2 = __shfl_sync(0xffffffffu, c1, (4 * lane + j) & 31), s2 = __shfl_sync(0xffffffffu, s1, (4 * lane + j) & 31);
+                    if (lane >> 3 == k) { cs[j] = c2; sn[j] = s2; }
+                }
             }
-        }
         if (p.norm_w && on) {
             float ss = 0.f;
 #pragma unroll
@@ -224,6 +237,7 @@ struct ka {
     float low[4];       // of this warp's rows, column g in two terms: sums of p lowest of groups 2 ft, 2 ft + 1; ft = 2: the sum of p
     float acc[8][2];    // of this warp's group and part, column g: features 8 (2 ft, 2 ft + 1) + j: of a for even j, of a + 16 b for odd ones
     uint32_t ref[S];    // fp16 bits, twice, of the scales that the groups' are taken against
+    uint32_t room[S];   // and of the largest that they may take
     uint32_t up[S];     // fp16 2^-1 over a reference's power of two, twice
     float f;            // of column g's scores
     int len, first_new; // rows of the item, the first of its new ones
@@ -236,7 +250,7 @@ struct ka {
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = 0.f;
 #pragma unroll
-        for (int q = 0; q < S; ++q) ref[q] = up[q] = 0u;
+        for (int q = 0; q < S; ++q) ref[q] = room[q] = up[q] = 0u;
     }
 
     // (scale, lowest) of four rows, of those that are there
@@ -267,20 +281,18 @@ struct ka {
         for (int i = 0; i < 4; ++i) pr[i] = ka_exp2(fmaf(r.sc[i], f, less));
         ka_split(pr[0], pr[1], r.hi.x, r.lo.x);
         ka_split(pr[2], pr[3], r.hi.y, r.lo.y);
+        uint32_t on01 = ~0u, on23 = ~0u;
+        if (edge) { // a NaN's group reaches the columns that see its row, and no other as 0 times NaN
+            const int lim = s.limit[g];
+            on01 = (row0 <= lim ? 0xffffu : 0u) | (row0 + 1 <= lim ? 0xffff0000u : 0u);
+            on23 = (row0 + 2 <= lim ? 0xffffu : 0u) | (row0 + 3 <= lim ? 0xffff0000u : 0u);
+        }
 #pragma unroll
         for (int q = 0; q < S; ++q) {
-            const __half2 u = *reinterpret_cast<const __half2*>(&up[q]);
-            const float2 s01 = __half22float2(__hmul2(*reinterpret_cast<const __half2*>(&r.s01[q]), u)), s23 = __half22float2(__hmul2(*reinterpret_cast<const __half2*>(&r.s23[q]), u));
-            float w[4] = {pr[0] * s01.x, pr[1] * s01.y, pr[2] * s23.x, pr[3] * s23.y};
-            if (edge) { // a NaN's group reaches the columns that see its row, and no other as 0 times NaN
-                const int lim = s.limit[g];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (row0 + i > lim) w[i] = 0.f;
-            }
+            // (hi + lo) scale in two terms: the first product rounded, what the rounding left exactly, and lo scale on top of that
             uint4 o;
-            ka_split(w[0], w[1], o.x, o.y);
-            ka_split(w[2], w[3], o.z, o.w);
+            ka_scale(r.hi.x, r.lo.x, edge ? r.s01[q] & on01 : r.s01[q], up[q], o.x, o.y);
+            ka_scale(r.hi.y, r.lo.y, edge ? r.s23[q] & on23 : r.s23[q], up[q], o.z, o.w);
             s.p[q][b][lane] = o;
         }
     }
@@ -348,7 +360,7 @@ struct ka {
                     r[k].s23[q] = __byte_perm(vr.z, vr.w, 0x5410);
                     // does something pass its reference by more than there is room for?  A reference of 0 has none
                     const uint32_t v = widest(r[k].s01[q], r[k].s23[q], edge);
-                    over |= v != __vminu2(v, ref[q] ? __vaddus2(ref[q], KA_WIDE) : 0u);
+                    over |= v != __vminu2(v, room[q]);
                 }
                 if (edge) {
                     const int lim = s.limit[g];
@@ -477,6 +489,7 @@ struct ka {
         for (int q = 0; q < S; ++q) {
             const uint32_t v = __byte_perm(q & 2 ? mx.y : mx.x, 0u, q & 1 ? 0x3232 : 0x1010), old = ref[q];
             ref[q] = __vmaxu2(old, v);
+            room[q] = ref[q] ? __vaddus2(ref[q], KA_WIDE) : 0u;
             const int e = ka_exponent(ref[q] & 0xffffu);
             if (q == warp % S) shrink = corr * ka_pow2(ka_exponent(old & 0xffffu) - e);
             const __half2 u = __float2half2_rn(ka_pow2(-1 - e));
@@ -577,6 +590,7 @@ struct ka {
             mbar_init(&s.pfree, KA_WARPS);
             mbar_fence_init();
         }
+        for (int i = t; i < p.rot_dims / 2; i += KA_THREADS) s.freq[i] = p.freq[i];
         pdl_wait();
         const uint32_t total = read_batch(); // its barriers also show the mbarriers to everybody
         const uint32_t ctas = min(gridDim.x, total);

@@ -558,6 +558,7 @@ typedef struct {
  * One record per sequence, KV head and 16 rows: LB_KV4_BLOCK(D) bytes, see kv4.cuh */
 #define LB_KV4_BLOCK(D) (18 * (D))
 #define LB_KV4_REQS 256   /* requests of a batch */
+#define LB_KV4_ROWS (1 << 24) /* token rows of a batch */
 #define LB_KV4_NEW 16     /* new tokens of a request in an attention call */
 typedef struct {
     unsigned char* cache;
@@ -605,7 +606,7 @@ typedef struct {
 #define LB_KV4_CTAS 2
 #define LB_KV4_MAX_CTAS 1024
 #define LB_KV4_STAGES 2
-#define LB_KV4_SMEM (LB_KV4_STAGES * 36864 + 16384 + 8192 + 8 * 1024)
+#define LB_KV4_SMEM (LB_KV4_STAGES * 36864 + 16384 + 8192 + 9 * 1024)
 
 /* ---- drafted tokens against the target's probabilities (verify.cu) -------------------------------------------- */
 #define LB_VD_REQS 256

@@ -133,20 +133,25 @@ def test_read_types(lb, ctx, kind, dim, heads):
 
 
 # ---- attention ----------------------------------------------------------------------------------------------------
-def attention(lb, ctx, case, G, kind, norm=False, rot=0, gate=False, max_new=None, seed=6, gap=0, size=1.0, change=None):
+def attention(lb, ctx, case, G, kind, norm=False, rot=0, gate=False, max_new=None, seed=6, gap=0, size=1.0, change=None, shift=0, gate_at=None, row_gap=0):
     """the call's result and its check against 64 bits; `change` may edit the queries (by reference)"""
     rng, D, H = np.random.default_rng(seed), case.dim, case.heads
-    HQ, width = H * G, D * (1 + gate) + gap
-    x = size * rng.standard_normal((case.rows, HQ, width))
+    HQ, at = H * G, D if gate_at is None else gate_at
+    width = (at + D if gate else D) + gap
+    x = size * rng.standard_normal((case.rows, HQ * width + row_gap))
     if change:
         change(x)
     raw, x = kc.typed(x, kind)
+    row_stride = x.shape[1]
+    raw, x = np.concatenate([np.zeros(shift, raw.dtype), raw.ravel()]), x[:, :HQ * width].reshape(case.rows, HQ, width)
     w = lb.f32_to_bf16((1 + 0.1 * rng.standard_normal(D)).astype(np.float32)) if norm else None
     d_x, d_w = ctx.to_device(raw), ctx.to_device(w) if norm else None
-    d_gate = type("At", (), {"ptr": d_x.ptr + D * raw.itemsize}) if gate else None
-    out = ctx.to_device(np.full(case.rows * HQ * D, 9.0, np.float16))
-    ctx.kv4_attention(case.desc, case.batch, d_x, d_gate, 0, width, kind, d_w, out, HQ, max_new or max(case.new), rot, THETA, EPS)
-    got = out.download(np.float16).astype(np.float64).reshape(case.rows, HQ, D)
+    where = lambda n: type("At", (), {"ptr": d_x.ptr + n * raw.itemsize})  # noqa: E731
+    out = ctx.to_device(np.full(shift + case.rows * HQ * D, 9.0, np.float16))
+    d_out = type("At", (), {"ptr": out.ptr + 2 * shift})
+    ctx.kv4_attention(case.desc, case.batch, where(shift), where(shift + at) if gate else None, row_stride if row_gap else 0, width, kind, d_w, d_out, HQ, max_new or max(case.new), rot,
+                      THETA, EPS)
+    got = out.download(np.float16)[shift:].astype(np.float64).reshape(case.rows, HQ, D)
     assert ctx.device_status() == 0
     worst, rows = 0.0, {}
     for row, seq, pos in case.places():
@@ -157,7 +162,7 @@ def attention(lb, ctx, case, G, kind, norm=False, rot=0, gate=False, max_new=Non
                 rows[seq, h // G] = n, kc.cache_rows(case.cache, D, seq, h // G, n)
             want, tol = kc.attend(q[h], *rows[seq, h // G][1], pos)
             if gate:
-                g = 1 / (1 + np.exp(-x[row, h, D:2 * D]))
+                g = 1 / (1 + np.exp(-x[row, h, at:at + D]))
                 want, tol = want * g, tol * g + np.abs(want * g) * 2.0 ** -20
             tol = tol + 2.0 ** -11 * (np.abs(want) + tol) + 2.0 ** -25  # the output's rounding
             err = np.abs(got[row, h] - want)
@@ -193,6 +198,31 @@ def test_attention_drafts(lb, ctx, dim, heads, G, new):
     """several new tokens see as many rows as their places allow; columns beyond one set of products"""
     case = kc.Case(ctx, dim, heads, 4, 528, seqs=[3, 1, 0], pos=[0, 500, 250], new=new)
     attention(lb, ctx, case, G, lb.IN_F32, norm=True, rot=64, gate=True)
+    case.free()
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+@pytest.mark.parametrize("shift,gap,row_gap,gate_at", [(0, 0, 0, 67), (1, 0, 0, 64), (0, 5, 3, 64), (0, 8, 16, 72), (3, 1, 1, 65), (8, 0, 0, 128)])
+def test_attention_alignments(lb, ctx, kind, shift, gap, row_gap, gate_at):
+    """queries, gates, rows and results at any place that their type allows, each for itself"""
+    case = kc.Case(ctx, 64, 2, 2, 256, seqs=[1, 0], pos=[200, 30], new=[2, 1])
+    attention(lb, ctx, case, 3, kind, True, 32, True, shift=shift, gap=gap, row_gap=row_gap, gate_at=gate_at)
+    case.free()
+
+
+def test_attention_most_columns(lb, ctx):
+    """16 heads on one, 16 new tokens: 32 passes over the rows"""
+    case = kc.Case(ctx, 128, 2, 2, 512, seqs=[1, 0], pos=[300, 0], new=[16, 3])
+    attention(lb, ctx, case, 16, lb.IN_F16, rot=128)
+    case.free()
+
+
+def test_attention_more_tiles_than_ctas(lb, ctx):
+    """items that begin, go on and end in every way in a CTA's share"""
+    rng = np.random.default_rng(12)
+    pos = rng.integers(0, 700, 40)
+    case = kc.Case(ctx, 64, 8, 40, 704, seqs=rng.permutation(40), pos=pos, new=[1] * 40)
+    attention(lb, ctx, case, 1, lb.IN_F32)
     case.free()
 
 
@@ -343,7 +373,7 @@ def test_refusals(lb, ctx):
     for i, v in ((0, 0), (0, b.ptr + 8), (1, 0), (2, 24), (2, 0), (3, 0), (3, 40), (4, 32), (4, 192)):
         for call, rest in ((ctx.kv4_append, (b, b)), (ctx.kv4_read, (b, b)), (ctx.kv4_attention, (b, None, 0, 0, 1, None, b, 1))):
             bad(call, desc(i, v), good[1], *rest)
-    for i, v in ((1, 0), (1, b.ptr + 2), (3, 0), (3, 257), (4, 0), (4, 2)):
+    for i, v in ((1, 0), (1, b.ptr + 2), (3, 0), (3, 257), (4, 0), (4, 2), (4, (1 << 24) + 1)):
         for call, rest in ((ctx.kv4_append, (b, b)), (ctx.kv4_read, (b, b)), (ctx.kv4_attention, (b, None, 0, 0, 1, None, b, 1))):
             bad(call, good[0], desc(i, v, batch, lb.Kv4Batch), *rest)
     null = type("At", (), {"ptr": 0})
