@@ -50,8 +50,7 @@ __device__ __forceinline__ double vd_double(float v) {
 }
 
 // exp of many differences l - max in 64 bits: y = (l - max) 256 / (T ln 2) = 256 a + j + f with |f| <= 1/2, exp = 2^a 2^(j/256) e^(f ln 2 / 256), the last factor by its series, whose
-// fourth term is below 2e-13.  Eight operations in 64 bits, which are what the pick's time goes into; the library's exp also serves arguments that do not occur here
-// and makes it twice as long.
+// fourth term is below 2e-13.  Eight operations in 64 bits, two issue slots each; the library's exp also serves arguments that do not occur here and makes the pick twice as long.
 #define VD_STEPS 256
 struct vd_exps {
     double scale, less; // y = l * scale - less
@@ -66,15 +65,32 @@ struct vd_exps {
         less = infinite ? 0.0 : (double)max * scale;
         low = infinite ? max : max > -INFINITY ? (float)fmax((double)max - 693.0 * temperature, -3.4028234e38) : NAN;
     }
-    __device__ __forceinline__ double operator()(float l) const {
+    // N at a time, step by step: every operation waits for the one before, so others have to be under way
+    template <int N>
+    __device__ __forceinline__ void operator()(const float (&l)[N], double (&e)[N]) const {
         constexpr double L = 0.69314718055994530942 / VD_STEPS, magic = 6755399441055744.0; // 1.5 * 2^52: what is added to it is rounded to a whole number
-        const double y = fma(vd_double(l), scale, -less), whole = y + magic, f = y - (whole - magic);
-        double e = fma(f, L * L * L / 6.0, L * L / 2.0);
-        e = fma(f, e, L);
-        e = fma(f, e, 1.0);
-        const int n = __double2loint(whole);
-        e *= table[n & (VD_STEPS - 1)];
-        return l >= low ? __hiloint2double(__double2hiint(e) + ((n >> 8) << 20), __double2loint(e)) : 0.0; // a NaN is not
+        double f[N];
+        int n[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = fma(vd_double(l[i]), scale, -less);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const double whole = f[i] + magic;
+            n[i] = __double2loint(whole);
+            e[i] = whole - magic;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] -= e[i];
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = fma(f[i], L * L * L / 6.0, L * L / 2.0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = fma(f[i], e[i], L);
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = fma(f[i], e[i], 1.0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] *= table[n[i] & (VD_STEPS - 1)];
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = l[i] >= low ? __hiloint2double(__double2hiint(e[i]) + ((n[i] >> 8) << 20), __double2loint(e[i])) : 0.0; // a NaN is not
     }
 };
 
@@ -477,7 +493,7 @@ extern "C" __global__ void __launch_bounds__(32) vd_pick_short(const __grid_cons
 // exponentials as they are (one pass); against the draft's probabilities they have to be divided by their sum first (a pass for it).  grid (requests, cluster)
 #define VP_THREADS 512
 #define VP_WARPS (VP_THREADS / 32)
-extern "C" __global__ void __launch_bounds__(VP_THREADS, 2) vd_pick(const __grid_constant__ lb_vd_params p) {
+extern "C" __global__ void __launch_bounds__(VP_THREADS, 1) vd_pick(const __grid_constant__ lb_vd_params p) {
     __shared__ double part[2];           // this CTA's sum: of the exponentials, of the weights
     __shared__ double ws[VP_WARPS], table[VD_STEPS];
     __shared__ int s_token, s_last;
@@ -495,7 +511,7 @@ extern "C" __global__ void __launch_bounds__(VP_THREADS, 2) vd_pick(const __grid
     const float* q = inner && p.probs ? p.probs + (size_t)at * p.V : nullptr;
     const int gone = inner && !p.probs ? p.drafts[at] : -1; // a certain draft
     const vd_exps expo(table, st.max, p.temperature);
-    const int per = (p.V + C * VP_WARPS - 1) / (C * VP_WARPS), a = min(p.V, (rank * VP_WARPS + warp) * per), b = min(p.V, a + per); // this warp's range
+    const int per = ((p.V + C * VP_WARPS - 1) / (C * VP_WARPS) + 3) & ~3, a = min(p.V, (rank * VP_WARPS + warp) * per), b = min(p.V, a + per); // this warp's range
     double sums[LB_VD_CLUSTER];
     auto all = [&](double v, int which) { // sum over the CTA into part[which] (ws: the warps'), then over the cluster in its order; sums: the CTAs'
 #pragma unroll
@@ -516,60 +532,72 @@ extern "C" __global__ void __launch_bounds__(VP_THREADS, 2) vd_pick(const __grid
         for (int c = 0; c < LB_VD_CLUSTER; ++c) s += sums[c];
         return s;
     };
-    // f(index, logit) or f(index, logit, q) over a warp's range, eight values of a lane in flight
-    auto over = [&](auto f) {
-        double s0 = 0.0, s1 = 0.0;
-        int i = a + lane;
-        for (; i + 224 < b; i += 256) {
-            float l[8];
+    // weights of four logits at i, i + step, ..: p; p without a certain draft; max(p - q, 0), a q that is no positive number being 0
+    auto plain = [&](int, int, const float (&l)[4], const float (&)[4], double (&w)[4]) { expo(l, w); };
+    auto without = [&](int i, int step, const float (&l)[4], const float (&)[4], double (&w)[4]) {
+        expo(l, w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) l[j] = __ldg(x + i + 32 * j);
+        for (int j = 0; j < 4; ++j)
+            if (i + j * step == gone) w[j] = 0.0;
+    };
+    auto rest = [&](int, int, const float (&l)[4], const float (&o)[4], double (&w)[4]) {
+        expo(l, w);
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                s0 += f(i + 32 * j, l[j]);
-                s1 += f(i + 32 * j + 32, l[j + 1]);
+        for (int j = 0; j < 4; ++j) {
+            const double d = w[j] - vd_double(fmaxf(o[j], 0.f));
+            w[j] = o[j] < INFINITY && __double2hiint(d) >= 0 ? d : o[j] >= 0.f ? 0.0 : w[j];
+        }
+    };
+    // their sum over a warp's range: four neighbours a lane and load, the next loads on their way while the values of the last ones are worked on
+    auto over = [&](auto f, const float* other) {
+        constexpr int H = 3;
+        double s[4] = {0.0, 0.0, 0.0, 0.0};
+        float4 l[H], o[H];
+        const bool wide = (((size_t)(x + a) | (other ? (size_t)(other + a) : 0)) & 15) == 0;
+        auto four = [&](const float* v, int i, float none) {
+            if (i + 3 < b && wide) return __ldg(reinterpret_cast<const float4*>(v + i));
+            return make_float4(i < b ? v[i] : none, i + 1 < b ? v[i + 1] : none, i + 2 < b ? v[i + 2] : none, i + 3 < b ? v[i + 3] : none);
+        };
+        auto load = [&](int i) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                l[h] = four(x, i + 128 * h, -INFINITY);
+                if (other) o[h] = four(other, i + 128 * h, 0.f);
+            }
+        };
+        load(a + 4 * lane);
+        for (int i = a + 4 * lane; i < a + 4 * lane + per; i += 128 * H) { // the whole warp goes on while any lane does
+            float4 l0[H], o0[H];
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                l0[h] = l[h];
+                o0[h] = other ? o[h] : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            load(i + 128 * H); // behind the range: nothing is read
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                if (i + 128 * h - 4 * lane >= b) break; // the same for the warp
+                const float lv[4] = {l0[h].x, l0[h].y, l0[h].z, l0[h].w}, ov[4] = {o0[h].x, o0[h].y, o0[h].z, o0[h].w};
+                double w[4];
+                f(i + 128 * h, 1, lv, ov, w);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j] += w[j];
             }
         }
-        for (; i < b; i += 32) s0 += f(i, x[i]);
-        return s0 + s1;
+        return (s[0] + s[1]) + (s[2] + s[3]);
     };
-    auto over2 = [&](auto f) {
-        double s0 = 0.0, s1 = 0.0;
-        int i = a + lane;
-        for (; i + 224 < b; i += 256) {
-            float l[8], o[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                l[j] = __ldg(x + i + 32 * j);
-                o[j] = __ldg(q + i + 32 * j);
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                s0 += f(l[j], o[j]);
-                s1 += f(l[j + 1], o[j + 1]);
-            }
-        }
-        for (; i < b; i += 32) s0 += f(x[i], q[i]);
-        return s0 + s1;
-    };
-    auto rest = [&](float l, float o) { // max(p - q, 0); a q that is no positive number is 0
-        const double e = expo(l), d = e - vd_double(fmaxf(o, 0.f));
-        return o < INFINITY && __double2hiint(d) >= 0 ? d : o >= 0.f ? 0.0 : e;
-    };
-    auto plain = [&](int, float l) { return expo(l); };
-    auto without = [&](int i, float l) { return i == gone ? 0.0 : expo(l); };
     double total;
     bool whole = !inner; // the weights are p
     if (q) {
-        const double z = 1.0 / all(over(plain), 0);
+        const double z = 1.0 / all(over(plain, nullptr), 0);
         for (int i = t; i < VD_STEPS; i += VP_THREADS) table[i] *= z; // from here on the exponentials are probabilities
         __syncthreads();
-        total = all(over2(rest), 1);
-    } else total = all(gone >= 0 ? over(without) : over(plain), 1);
+        total = all(over(rest, q), 1);
+    } else total = all(gone >= 0 ? over(without, nullptr) : over(plain, nullptr), 1);
     if (!whole && !(total > 0.0)) { // rounding left nothing: from p itself
         whole = true;
         cluster.sync(); // the sums have been read
-        total = all(over(plain), 1);
+        total = all(over(plain, nullptr), 1);
     }
     cluster.sync(); // nobody leaves while its sums are read
     const double goal = (double)p.u_pick[r] * total;
@@ -603,16 +631,17 @@ extern "C" __global__ void __launch_bounds__(VP_THREADS, 2) vd_pick(const __grid
     const int lo = min(p.V, (rank * VP_WARPS + w0) * per), hi = min(p.V, lo + per);
     for (int i0 = lo; i0 < hi; i0 += 4 * VP_THREADS) {
         const int i = i0 + 4 * t;
-        double v[4], run = 0.0;
+        float l[4], o[4];
+        double v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            v[j] = 0.0;
-            if (i + j < hi) {
-                const float l = x[i + j];
-                v[j] = whole ? expo(l) : q ? rest(l, q[i + j]) : without(i + j, l);
-            }
-            run += v[j];
+            l[j] = i + j < hi ? x[i + j] : -INFINITY;
+            o[j] = q && i + j < hi ? q[i + j] : 0.f;
         }
+        if (whole) plain(i, 1, l, o, v);
+        else if (q) rest(i, 1, l, o, v);
+        else without(i, 1, l, o, v);
+        double run = (v[0] + v[1]) + (v[2] + v[3]);
         const double mine = run;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
