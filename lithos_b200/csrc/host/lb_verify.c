@@ -7,7 +7,7 @@ static unsigned cluster_of(int n, int vocab, int slots) {
     int best = 1;
     double least = 1e30;
     for (int k = 1; k <= LB_VD_CLUSTER && (k == 1 || vocab / k >= 4096); k++) {
-        const double time = (double)((n * k + slots - 1) / slots) * (1.0 / k + 0.03); /* waves of a share and of what a CTA costs besides */
+        const double time = (double)((n * k + slots - 1) / slots) * (1.0 / k + 0.06); /* waves of a share and of what a CTA costs besides */
         if (time < least) { least = time; best = k; }
     }
     return (unsigned)best;
