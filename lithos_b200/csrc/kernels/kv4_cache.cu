@@ -40,13 +40,22 @@ __device__ __forceinline__ uint32_t kc_codes(const double (&x)[8], double lo, fl
     constexpr double magic = 6755399441055744.0; // 1.5 * 2^52: what is added to it is rounded to a whole number
     const double s = (double)scale, guess = (double)(1.0f / scale), inv = fma(guess, fma(-s, guess, 1.0), guess);
     uint32_t word = 0;
+    bool near = false;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const double d = x[j] - lo, y = d * inv;
-        double n = y + magic;
-        const double off = y - (n - magic);
-        if ((__double2hiint(off) & 0x7fffffff) >= 0x3fdffffe) n = d / s + magic; // |off| >= 1/2 - 2^-21
+        const double y = (x[j] - lo) * inv, n = y + magic;
+        near |= (__double2hiint(y - (n - magic)) & 0x7fffffff) >= 0x3fdffffe; // 1/2 - 2^-21 or more off
         word |= (uint32_t)min(max(__double2loint(n), 0), 15) << (4 * j);
+    }
+    if (near) {
+        word = 0;
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+            double v = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) v = j == i ? x[i] : v;
+            word |= (uint32_t)min(max(__double2loint((v - lo) / s + magic), 0), 15) << (4 * j);
+        }
     }
     return word;
 }
@@ -124,16 +133,25 @@ __device__ __forceinline__ void kv4_append_body(const lb_kv4_rows_params& p) {
                     }
                 }
             }
-            float lo_f = INFINITY; // rounding keeps the order: the least of the rounded values is the least value rounded
+            float lo_f = INFINITY, size = 0.f, none = 0.f; // rounding keeps the order: the least of the rounded values is the least value rounded
             double hi = 0.0;
             bool bad = false;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float v = part ? in[j] : (float)x[j];
-                bad |= !(fabsf(v) < INFINITY) && !(fabs(x[j]) <= 1.7976931348623157e308);
-                if (fabsf(v) > 65504.f) x[j] = v > 0.f ? 65504.0 : -65504.0; // what fp16 holds: a value beyond it is cut off
                 lo_f = fminf(lo_f, v);
+                size = fmaxf(size, fabsf(v));
+                none = fmaf(v, 0.f, none); // a NaN if one of them is, or is infinite
                 hi = j == 0 || x[j] > hi ? x[j] : hi;
+            }
+            if (size > 65504.f || none != 0.f) { // what fp16 holds: a value beyond it is cut off
+                hi = -65504.0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    bad |= !(fabs(x[j]) <= 1.7976931348623157e308);
+                    x[j] = fmin(fmax(x[j], -65504.0), 65504.0);
+                    hi = fmax(hi, x[j]);
+                }
             }
 #pragma unroll
             for (int o = 4; o > 0; o >>= 1) {
