@@ -57,7 +57,7 @@ int lb_device_sm_count(const lb_ctx* ctx);
  * when it is non-zero, returns LB_ERR_DEVICE_WAIT and clears the word.  The reference's own bounded wait traps the
  * GPU instead (runtime/sync.ls:50-60 sync_wait_flag_timeout); here the kernel returns and the host reads why:
  * 0x1001 a weight copy never landed, 0x1003 a peer GPU never published its flag, 0x1004 a CTA never reached the grid
- * barrier, 0x1005 the decode position lies outside the KV cache. */
+ * barrier, 0x1005 the decode position (a request's rows) lies outside the KV cache, 0x1006 a request of a batch names token rows or a sequence that are not there. */
 int lb_device_status(lb_ctx* ctx, uint32_t* status_out);
 int lb_reset_status(lb_ctx* ctx); /* clear the status word without reading it (stream-ordered) */
 /* Time limit, in nanoseconds, of the kernels' waits on other CTAs and other GPUs (grid barrier, peer flags); 0 = the
@@ -308,7 +308,7 @@ int lb_kv4_append(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* ba
 int lb_kv4_read(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t k_out, uint64_t v_out, int type);
 /* Attention of the batch's new tokens, whose rows are in the cache: token i of request r sees rows 0 .. pos[r] + i.
  * q and gate (0: none): element type `type`, head h of token row j at j * row_stride + h * head_stride elements (row_stride 0: n_heads * head_stride, head_stride 0: dim); q is
- * normalised per head (q_norm_w; 0: not) and rotated like the keys, then rounded to fp16; the result is multiplied by sigmoid(gate).  n_heads: 1 to 16 times
+ * normalised per head (q_norm_w; 0: not) and rotated like the keys, and goes in with 22 bits; the result is multiplied by sigmoid(gate).  n_heads: 1 to 16 times
  * kv_heads.  max_new: the most tokens a request of the batch has, 1 .. LB_KV4_MAX_NEW.  out fp16 [rows, n_heads, dim], what lb_gemm_int4 takes; it
  * overlaps none of the inputs. */
 int lb_kv4_attention(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t q, uint64_t gate, int64_t row_stride, int64_t head_stride, int type,
@@ -321,7 +321,7 @@ int lb_kv4_attention(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch*
  * draft where draft_probs = 0 (drafts that were not drawn).  Logits of -infinity or NaN have probability 0.
  *   Row by row a draft x stands while  u_accept[row] * q(x) < p(x)  (greedy: while it is the arg-max).  The first row that does not stand, or the last one, gives the token: the
  * first one, by index (top_k: by rank), at which the running sum of weights exceeds u_pick[r] times the whole, weights max(p - q, 0), at the last row p (and where the former are all
- * 0).  All of that is computed in 64 bits.
+ * 0).  Probabilities and sums that choose the token are computed in 64 bits; the p that a draft is held against, over the whole vocabulary, to about 2^-20 of itself.
  * tokens i32 [rows]: the drafts that stand, the token, then -1; accepted i32 [n_reqs]: how many stand, -1 for a request without rows; p_out fp32 [rows] (0: not wanted):
  * p of every draft, 0 in last rows.  Rows behind the last request's are left as they were; a request that names rows that are not there gets -1, status word 0x1006. */
 enum { LB_VERIFY_MAX_REQS = 256, LB_VERIFY_MAX_ROWS = 8192 };
