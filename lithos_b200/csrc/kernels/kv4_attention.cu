@@ -14,7 +14,8 @@
 //     16 rows, leaves p scale in shared memory as operands, and adds up a group's 64 features over its part of the tile.  References are standing: probabilities are
 //     taken against the largest score, and weights against the largest scale, at the last time that a score passed its reference by 2^6 or a scale by 2^5, for which
 //     fp16 has room; so a tile usually costs one barrier and no exchange of maxima.
-//   * All tiles of all items are dealt evenly to the CTAs in one line, so that ragged batches balance; an item cut by a border leaves records that kv4_merge joins in order.
+//   * All tiles of all items are dealt evenly to the CTAs in one line, with a place more for an item's start and end, so that ragged batches balance; an item cut by a border
+//     leaves records that kv4_merge joins in order.
 // mma.sync rather than tcgen05: the columns are few (6 for one token of 24 heads on 4), and codes would have to be widened into shared or tensor memory for it.
 // Bound by three things at once: per tile and SM, some 800 instructions a warp (issue slots 50 - 60 % busy), 200 passes through shared memory a warp (two thirds of its time: queries 64,
 // copies in 36, codes 32, weights out and in 32, scales 36) and the tensor pipe (35 - 40 %); what overlaps them is 16 warps an SM, as many as 128 registers leave.
@@ -93,7 +94,7 @@ struct ka {
         float factor[KA_COLS], m[KA_COLS], l[KA_COLS], low[KA_COLS][S];
         uint64_t full[NS], pfree;
         ka_item ahead;                  // the last tile that was requested
-        uint32_t pre[LB_KV4_REQS + 1];  // tiles before request r
+        uint32_t pre[LB_KV4_REQS + 1];  // places in the line before request r
         int len[LB_KV4_REQS], n[LB_KV4_REQS], start[LB_KV4_REQS], seq[LB_KV4_REQS], limit[KA_COLS];
         uint32_t requested, warp_sum[KA_WARPS]; // requested: tiles of this CTA
     };
@@ -106,13 +107,14 @@ struct ka {
 
     __device__ __forceinline__ int sets(int n) const { return (n * G + KA_COLS - 1) / KA_COLS; }
 
-    // the requests, and how many tiles lie before each
+    // The line of work: for every item (request, KV head, set of columns) a place for its queries and its results, which take about as long as a tile, and one for every tile.
+    // the requests, and how many places lie before each
     __device__ __forceinline__ uint32_t read_batch() {
         kv4_request q = {0, 0, 0, 0};
         if (t < p.b.n_reqs) q = kv4_get(p.b, t);
         const int len = q.n > 0 ? q.pos + q.n : 0;
         s.len[t] = len; s.n[t] = q.n; s.start[t] = q.start; s.seq[t] = q.seq;
-        uint32_t sum = q.n > 0 ? (uint32_t)((len + TILE - 1) / TILE) * p.b.HKV * sets(q.n) : 0u;
+        uint32_t sum = q.n > 0 ? (uint32_t)((len + TILE - 1) / TILE + 1) * p.b.HKV * sets(q.n) : 0u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -131,6 +133,7 @@ struct ka {
         __syncthreads();
         return total;
     }
+    // the first tile at place x of the line, or behind it where x is an item's first place
     __device__ __forceinline__ ka_item place(uint32_t x) const {
         int lo = 0, hi = p.b.n_reqs - 1; // the last request with pre <= x that has tiles
         while (lo < hi) {
@@ -141,11 +144,30 @@ struct ka {
         ka_item it;
         it.r = lo;
         it.tiles = (s.len[lo] + TILE - 1) / TILE;
-        const int local = (int)(x - s.pre[lo]), item = local / it.tiles, z = sets(s.n[lo]);
-        it.tile = local - item * it.tiles;
+        const int local = (int)(x - s.pre[lo]), item = local / (it.tiles + 1), z = sets(s.n[lo]);
+        it.tile = max(local - item * (it.tiles + 1) - 1, 0);
         it.kv = item / z;
         it.z = item - it.kv * z;
         return it;
+    }
+    // how many of the places x0 .. x1 - 1 are tiles, from the item that x0 falls into
+    __device__ __forceinline__ uint32_t tiles_of(uint32_t x0, uint32_t x1) const {
+        int r = 0;
+        uint32_t n = x1 - x0;
+        {
+            int hi = p.b.n_reqs - 1;
+            while (r < hi) {
+                const int mid = (r + hi + 1) >> 1;
+                if (s.pre[mid] <= x0) r = mid;
+                else hi = mid - 1;
+            }
+        }
+        for (; r < p.b.n_reqs && s.pre[r] < x1; ++r) { // places at multiples of tiles + 1 from a request's first are not tiles
+            if (s.pre[r + 1] <= max(s.pre[r], x0)) continue;
+            const uint32_t one = (uint32_t)((s.len[r] + TILE - 1) / TILE) + 1u, from = max(x0, s.pre[r]) - s.pre[r], to = min(x1, s.pre[r + 1]) - s.pre[r];
+            n -= (to + one - 1) / one - (from + one - 1) / one;
+        }
+        return n;
     }
     __device__ __forceinline__ void next(ka_item& it) const {
         if (++it.tile < it.tiles) return;
@@ -605,13 +627,30 @@ struct ka {
             if (t == 0) join->first = -1;
             return;
         }
-        const uint32_t share = total / ctas, more = total - share * ctas; // the first `more` CTAs have one tile more
-        const uint32_t x0 = blockIdx.x * share + min(blockIdx.x, more), x1 = x0 + share + (blockIdx.x < more);
-        ka_item it = place(x0);
+        const uint32_t share = total / ctas, more = total - share * ctas; // the first `more` CTAs have one place more
+        const uint32_t from = blockIdx.x * share + min(blockIdx.x, more), to = from + share + (blockIdx.x < more), x1 = tiles_of(from, to);
+        ka_item it = place(from);
+        if (t == 32) { // does an item begin in the CTA before and go on here?  (another warp than the copies')
+            lb_kv4_join j;
+            j.first = -1;
+            if (x1 && it.tile > 0) {
+                const uint32_t begin = from - (uint32_t)it.tile, last = begin + (uint32_t)it.tiles - 1u; // places of its first and last tile
+                if (begin >= from - share - (blockIdx.x - 1 < more)) {
+                    j.first = (int)blockIdx.x - 1;
+                    j.last = (int)(last < more * (share + 1) ? last / (share + 1) : more + (last - more * (share + 1)) / share);
+                    j.row0 = s.start[it.r];
+                    j.kv = it.kv;
+                    j.col0 = it.z * KA_COLS;
+                    j.cols = min(KA_COLS, s.n[it.r] * G - j.col0);
+                }
+            }
+            *join = j;
+        }
+        if (!x1) return; // an item's first place alone
         if (t == 0) {
             ka_item a = it;
             uint32_t i = 0;
-            for (; i < NS && i < x1 - x0; ++i) {
+            for (; i < NS && i < x1; ++i) {
                 if (i) next(a);
                 copy(a, i);
             }
@@ -619,39 +658,24 @@ struct ka {
             s.requested = i;
         }
         bool first = true;
-        for (uint32_t x = x0; x < x1; ++x) {
-            if (x == x0 || it.tile == 0) {
+        for (uint32_t x = 0; x < x1; ++x) {
+            if (x == 0 || it.tile == 0) {
                 first = it.tile == 0;
                 queries(it);
                 begin(it);
                 __syncthreads();
                 f = s.factor[g];
             }
-            if (!tile(it, x - x0, x1 - x0)) { // a copy never landed: say so, let the others land, leave
+            if (!tile(it, x, x1)) { // a copy never landed: say so, let the others land, leave
                 if (t == 0) {
                     atomicExch(p.b.status, KV_FAIL_FULL);
-                    for (uint32_t y = x - x0; y < s.requested; ++y) mbar_wait(&s.full[y % NS], (y / NS) & 1);
+                    for (uint32_t y = x; y < s.requested; ++y) mbar_wait(&s.full[y % NS], (y / NS) & 1);
                 }
                 __syncthreads();
                 return;
             }
             if (it.tile == it.tiles - 1 || x == x1 - 1) finish(it, first, it.tile == it.tiles - 1);
             if (x + 1 < x1) next(it);
-        }
-        if (t == 0) { // does an item begin in the CTA before and go on here?
-            const ka_item at = place(x0);
-            lb_kv4_join j;
-            j.first = -1;
-            const uint32_t begin = x0 - (uint32_t)at.tile, end = begin + (uint32_t)at.tiles;
-            if (at.tile > 0 && begin >= x0 - share - (blockIdx.x - 1 < more)) {
-                j.first = (int)blockIdx.x - 1;
-                j.last = (int)(end - 1 < more * (share + 1) ? (end - 1) / (share + 1) : more + (end - 1 - more * (share + 1)) / share); // the CTA of tile end - 1
-                j.row0 = s.start[at.r];
-                j.kv = at.kv;
-                j.col0 = at.z * KA_COLS;
-                j.cols = min(KA_COLS, s.n[at.r] * G - j.col0);
-            }
-            *join = j;
         }
     }
 };
@@ -666,22 +690,30 @@ KA_KERNEL(64)
 KA_KERNEL(128)
 KA_KERNEL(256)
 
-// Joins the records of the items that were cut.  Every CTA counts the joins' columns; (join, column) pairs are dealt to groups of D / 4 threads, or to whole CTAs in which such
-// groups take runs of neighbouring records where there are few.  Records are added in the order of the rows, so results are the same from run to run.
+// Joins the records of the items that were cut.  Every CTA counts the joins' columns; a unit is 64 features of a column, for 16 threads: dealt to groups of 16, or to whole CTAs in which
+// the groups take runs of neighbouring records where there are few.  Records are added in the order of the rows, so results are the same from run to run.
 #define KM_THREADS 256
+#define KM_GROUPS (KM_THREADS / 16)
+__device__ __forceinline__ void km_add(float4& A, float& L, float4 a, float l, float w) {
+    L = fmaf(l, w, L);
+    A.x = fmaf(a.x, w, A.x); A.y = fmaf(a.y, w, A.y); A.z = fmaf(a.z, w, A.z); A.w = fmaf(a.w, w, A.w);
+}
 template <int D>
 __device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int ctas) {
-    constexpr int W = D / 4, SUB = KM_THREADS / W; // threads of a group, groups
+    constexpr int S = D / 64;
     __shared__ float4 red[KM_THREADS];
-    __shared__ float red_m[SUB], red_l[SUB];
+    __shared__ float red_m[KM_GROUPS], red_l[KM_GROUPS];
     __shared__ int pre[LB_KV4_MAX_CTAS + 1], s_warp[KM_THREADS / 32];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, sub = t / W, f = t % W * 4, G = p.HQ / p.b.HKV;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, sub = t >> 4, G = p.HQ / p.b.HKV;
     pdl_wait();
     int base = 0;
     if (t == 0) pre[0] = 0;
     for (int c0 = 0; c0 < ctas; c0 += KM_THREADS) { // columns before every join
         int sum = 0;
-        if (c0 + t < ctas && p.joins[c0 + t].first >= 0) sum = p.joins[c0 + t].cols;
+        if (c0 + t < ctas) {
+            const int first = p.joins[c0 + t].first, cols = p.joins[c0 + t].cols;
+            sum = first >= 0 ? cols : 0;
+        }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -699,81 +731,73 @@ __device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int 
         base += all;
         __syncthreads();
     }
-    const int pairs = base;
-    const bool few = pairs <= (int)gridDim.x; // a CTA for each
-    for (int first = few ? (int)blockIdx.x : (int)blockIdx.x * SUB; first < pairs; first += few ? (int)gridDim.x : (int)gridDim.x * SUB) {
-        const int pair = few ? first : first + sub;
+    const int units = base * S;
+    const bool few = units <= (int)gridDim.x; // a CTA for each
+    for (int first = few ? (int)blockIdx.x : (int)blockIdx.x * KM_GROUPS; first < units; first += few ? (int)gridDim.x : (int)gridDim.x * KM_GROUPS) {
+        const int unit = few ? first : first + sub, pair = unit / S, f = unit % S * 64 + (t & 15) * 4;
         float M = -INFINITY, L = 0.f;
-        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-        lb_kv4_join j;
-        int c = 0;
-        if (pair < pairs) {
+        float4 A = make_float4(0.f, 0.f, 0.f, 0.f), gate = A;
+        uint16_t* out = nullptr;
+        if (unit < units) {
             int lo = 0, hi = ctas - 1; // the last join with pre <= pair
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
                 if (pre[mid] <= pair) lo = mid;
                 else hi = mid - 1;
             }
-            j = p.joins[lo];
-            c = pair - pre[lo];
-            const int n = j.last - j.first + 1, per = few ? (n + SUB - 1) / SUB : n, b0 = j.first + (few ? sub * per : 0), b1 = min(j.last + 1, b0 + per);
+            const lb_kv4_join j = p.joins[lo];
+            const int c = pair - pre[lo], col = j.col0 + c, i = col / G, h = j.kv * G + col - i * G;
+            const size_t row = (size_t)(j.row0 + i);
+            const int n = j.last - j.first + 1, per = few ? (n + KM_GROUPS - 1) / KM_GROUPS : n, b0 = j.first + (few ? sub * per : 0), b1 = min(j.last + 1, b0 + per);
+            if (!few || sub == 0) {
+                out = p.out + (row * p.HQ + h) * D + f;
+                if (p.gate) {
+                    const size_t at = row * (size_t)p.row_stride + (size_t)h * (size_t)p.head_stride + f;
+                    gate = make_float4(kv4_load1(p.gate, at, p.type), kv4_load1(p.gate, at + 1, p.type), kv4_load1(p.gate, at + 2, p.type), kv4_load1(p.gate, at + 3, p.type));
+                }
+            }
             for (int b = b0; b < b1; b += 8) {
                 float mv[8], lv[8], mx = M;
                 float4 av[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool on = b + i < b1;
-                    const float* rec = p.records + (((size_t)(on ? b + i : b) * 2 + (b + i == j.first ? 1 : 0)) * KA_COLS + c) * LB_KV4_REC(D);
-                    mv[i] = on ? __ldcg(rec + D) : -INFINITY;
-                    lv[i] = on ? __ldcg(rec + D + 1) : 0.f;
-                    av[i] = on ? __ldcg(reinterpret_cast<const float4*>(rec + f)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int k = 0; k < 8; ++k) {
+                    const bool on = b + k < b1;
+                    const float* rec = p.records + (((size_t)(on ? b + k : b) * 2 + (b + k == j.first ? 1 : 0)) * KA_COLS + c) * LB_KV4_REC(D);
+                    mv[k] = on ? __ldcg(rec + D) : -INFINITY;
+                    lv[k] = on ? __ldcg(rec + D + 1) : 0.f;
+                    av[k] = on ? __ldcg(reinterpret_cast<const float4*>(rec + f)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, mv[i]);
+                for (int k = 0; k < 8; ++k) mx = fmaxf(mx, mv[k]);
                 const float use = mx == -INFINITY ? 0.f : mx, w = ka_exp2(M - use);
                 L *= w;
                 A.x *= w; A.y *= w; A.z *= w; A.w *= w;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = ka_exp2(mv[i] - use);
-                    L = fmaf(lv[i], v, L);
-                    A.x = fmaf(av[i].x, v, A.x); A.y = fmaf(av[i].y, v, A.y); A.z = fmaf(av[i].z, v, A.z); A.w = fmaf(av[i].w, v, A.w);
-                }
+                for (int k = 0; k < 8; ++k) km_add(A, L, av[k], lv[k], ka_exp2(mv[k] - use));
                 M = mx;
             }
         }
         if (few) {
             red[t] = A;
-            if (t % W == 0) { red_m[sub] = M; red_l[sub] = L; }
+            if ((t & 15) == 0) { red_m[sub] = M; red_l[sub] = L; }
             __syncthreads();
             if (sub == 0) {
-                float mx = M;
 #pragma unroll
-                for (int q = 1; q < SUB; ++q) mx = fmaxf(mx, red_m[q]);
-                const float use = mx == -INFINITY ? 0.f : mx;
+                for (int q = 1; q < KM_GROUPS; ++q) M = fmaxf(M, red_m[q]);
+                const float use = M == -INFINITY ? 0.f : M;
                 L = 0.f;
                 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int q = 0; q < SUB; ++q) {
-                    const float v = ka_exp2(red_m[q] - use);
-                    const float4 x = red[q * W + t];
-                    L = fmaf(red_l[q], v, L);
-                    A.x = fmaf(x.x, v, A.x); A.y = fmaf(x.y, v, A.y); A.z = fmaf(x.z, v, A.z); A.w = fmaf(x.w, v, A.w);
-                }
+                for (int q = 0; q < KM_GROUPS; ++q) km_add(A, L, red[q * 16 + t], red_l[q], ka_exp2(red_m[q] - use));
             }
             __syncthreads();
         }
-        if (pair < pairs && (!few || sub == 0)) {
-            const int col = j.col0 + c, i = col / G, h = j.kv * G + col - i * G;
-            const size_t row = (size_t)(j.row0 + i);
+        if (out) {
             const float inv = 1.f / L;
             float v[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
-            uint16_t* d = p.out + (row * p.HQ + h) * D + f;
+            if (p.gate) { v[0] *= sigmoidf_dev(gate.x); v[1] *= sigmoidf_dev(gate.y); v[2] *= sigmoidf_dev(gate.z); v[3] *= sigmoidf_dev(gate.w); }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (p.gate) v[k] *= sigmoidf_dev(kv4_load1(p.gate, row * (size_t)p.row_stride + (size_t)h * (size_t)p.head_stride + f + k, p.type));
-                d[k] = __half_as_ushort(__float2half_rn(v[k]));
-            }
+            for (int k = 0; k < 4; ++k) out[k] = __half_as_ushort(__float2half_rn(v[k]));
         }
     }
 }
