@@ -97,8 +97,8 @@ LB_API int lb_kv4_attention(lb_ctx* c, const lb_kv4_cache* cache, const lb_kv4_b
     p.HQ = n_heads; p.type = type; p.rot_dims = rot_dims; p.eps = eps;
     p.wide = ((q | gate | (uint64_t)row_stride * (uint64_t)size_of(type) | (uint64_t)head_stride * (uint64_t)size_of(type)) & 15) == 0;
     p.out_wide = out % 16 == 0;
-    /* no more CTAs than places in the line that a full cache would make */
-    const int64_t most = (int64_t)batch->n_reqs * HKV * sets * ((cache->max_ctx + LB_KV4_TILE(D) - 1) / LB_KV4_TILE(D) + 1);
+    /* no more CTAs than full sequences have work for */
+    const int64_t most = (int64_t)batch->n_reqs * HKV * sets * ((cache->max_ctx + LB_KV4_TILE(D) - 1) / LB_KV4_TILE(D) + 2);
     int ctas = c->sm_count * LB_KV4_CTAS < LB_KV4_MAX_CTAS ? c->sm_count * LB_KV4_CTAS : LB_KV4_MAX_CTAS;
     if (ctas > most) ctas = (int)most;
     void* params[] = {&p, &ctas};

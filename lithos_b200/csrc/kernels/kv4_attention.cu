@@ -14,7 +14,7 @@
 //     16 rows, leaves p scale in shared memory as operands, and adds up a group's 64 features over its part of the tile.  References are standing: probabilities are
 //     taken against the largest score, and weights against the largest scale, at the last time that a score passed its reference by 2^6 or a scale by 2^5, for which
 //     fp16 has room; so a tile usually costs one barrier and no exchange of maxima.
-//   * All tiles of all items are dealt evenly to the CTAs in one line, with a place more for an item's start and end, so that ragged batches balance; an item cut by a border
+//   * All tiles of all items are dealt evenly to the CTAs in one line, with places for an item's start and end, so that ragged batches balance; an item cut by a border
 //     leaves records that kv4_merge joins in order.
 // mma.sync rather than tcgen05: the columns are few (6 for one token of 24 heads on 4), and codes would have to be widened into shared or tensor memory for it.
 // Bound by three things at once: per tile and SM, some 800 instructions a warp (issue slots 50 - 60 % busy), 200 passes through shared memory a warp (two thirds of its time: queries 64,
@@ -74,6 +74,8 @@ __device__ __forceinline__ int ka_exponent(uint32_t bits) { return max((int)(bit
 
 struct ka_item { int r, kv, z, tile, tiles; }; // a place in the line of tiles
 
+#define KA_STEP 2u // places of a tile in the line of work
+#define KA_ITEM 3u // and of an item's queries and results in front of its tiles
 #define KA_LIFT 4.f  // probabilities are 2^4 at their reference
 #define KA_OVER 6.f  // and may pass it by 2^6
 #define KA_WIDE 0x14001400u // a scale may pass its group's reference by 2^5: fp16 bits
@@ -107,14 +109,16 @@ struct ka {
 
     __device__ __forceinline__ int sets(int n) const { return (n * G + KA_COLS - 1) / KA_COLS; }
 
-    // The line of work: for every item (request, KV head, set of columns) a place for its queries and its results, which take about as long as a tile, and one for every tile.
+    // The line of work: for every item (request, KV head, set of columns) KA_ITEM places for its queries and its results, which take about one and a half times as long as a tile, and
+    // KA_STEP for every tile, which belongs to the CTA that has its first.
+    __device__ __forceinline__ uint32_t places(int tiles) const { return KA_STEP * (uint32_t)tiles + KA_ITEM; }
     // the requests, and how many places lie before each
     __device__ __forceinline__ uint32_t read_batch() {
         kv4_request q = {0, 0, 0, 0};
         if (t < p.b.n_reqs) q = kv4_get(p.b, t);
         const int len = q.n > 0 ? q.pos + q.n : 0;
         s.len[t] = len; s.n[t] = q.n; s.start[t] = q.start; s.seq[t] = q.seq;
-        uint32_t sum = q.n > 0 ? (uint32_t)((len + TILE - 1) / TILE + 1) * p.b.HKV * sets(q.n) : 0u;
+        uint32_t sum = q.n > 0 ? places((len + TILE - 1) / TILE) * p.b.HKV * sets(q.n) : 0u;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
@@ -133,39 +137,41 @@ struct ka {
         __syncthreads();
         return total;
     }
-    // the first tile at place x of the line, or behind it where x is an item's first place
-    __device__ __forceinline__ ka_item place(uint32_t x) const {
-        int lo = 0, hi = p.b.n_reqs - 1; // the last request with pre <= x that has tiles
+    __device__ __forceinline__ int request_at(uint32_t x) const { // the last request with pre <= x that has tiles
+        int lo = 0, hi = p.b.n_reqs - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (s.pre[mid] <= x) lo = mid;
             else hi = mid - 1;
         }
+        return lo;
+    }
+    // the first tile that begins at place x of the line or behind it; base: the first place of the item that x lies in
+    __device__ __forceinline__ ka_item place(uint32_t x, uint32_t& base) const {
         ka_item it;
-        it.r = lo;
-        it.tiles = (s.len[lo] + TILE - 1) / TILE;
-        const int local = (int)(x - s.pre[lo]), item = local / (it.tiles + 1), z = sets(s.n[lo]);
-        it.tile = max(local - item * (it.tiles + 1) - 1, 0);
-        it.kv = item / z;
-        it.z = item - it.kv * z;
+        it.r = request_at(x);
+        it.tiles = (s.len[it.r] + TILE - 1) / TILE;
+        const uint32_t each = places(it.tiles), item = (x - s.pre[it.r]) / each, z = (uint32_t)sets(s.n[it.r]);
+        base = s.pre[it.r] + item * each;
+        it.kv = (int)(item / z);
+        it.z = (int)item - it.kv * (int)z;
+        it.tile = before(x - base);
+        if (it.tile == it.tiles) {
+            --it.tile;
+            next(it);
+        }
         return it;
     }
-    // how many of the places x0 .. x1 - 1 are tiles, from the item that x0 falls into
+    // how many tiles of an item begin before its place v
+    static __device__ __forceinline__ int before(uint32_t v) { return v <= KA_ITEM ? 0 : (int)((v - KA_ITEM + KA_STEP - 1) / KA_STEP); }
+    // how many tiles begin at places x0 .. x1 - 1
     __device__ __forceinline__ uint32_t tiles_of(uint32_t x0, uint32_t x1) const {
-        int r = 0;
-        uint32_t n = x1 - x0;
-        {
-            int hi = p.b.n_reqs - 1;
-            while (r < hi) {
-                const int mid = (r + hi + 1) >> 1;
-                if (s.pre[mid] <= x0) r = mid;
-                else hi = mid - 1;
-            }
-        }
-        for (; r < p.b.n_reqs && s.pre[r] < x1; ++r) { // places at multiples of tiles + 1 from a request's first are not tiles
+        uint32_t n = 0;
+        for (int r = request_at(x0); r < p.b.n_reqs && s.pre[r] < x1; ++r) {
             if (s.pre[r + 1] <= max(s.pre[r], x0)) continue;
-            const uint32_t one = (uint32_t)((s.len[r] + TILE - 1) / TILE) + 1u, from = max(x0, s.pre[r]) - s.pre[r], to = min(x1, s.pre[r + 1]) - s.pre[r];
-            n -= (to + one - 1) / one - (from + one - 1) / one;
+            const int tiles = (s.len[r] + TILE - 1) / TILE;
+            const uint32_t each = places(tiles), from = max(x0, s.pre[r]) - s.pre[r], to = min(x1, s.pre[r + 1]) - s.pre[r], i0 = from / each, i1 = to / each;
+            n += (i1 - i0) * (uint32_t)tiles + (uint32_t)before(to - i1 * each) - (uint32_t)before(from - i0 * each);
         }
         return n;
     }
@@ -621,7 +627,7 @@ struct ka {
         for (int i = t; i < p.rot_dims / 2; i += KA_THREADS) s.freq[i] = p.freq[i];
         pdl_wait();
         const uint32_t total = read_batch(); // its barriers also show the mbarriers to everybody
-        const uint32_t ctas = min(gridDim.x, total);
+        const uint32_t ctas = min(gridDim.x, total / KA_STEP); // whoever has places within an item has a tile of it
         lb_kv4_join* join = p.joins + blockIdx.x;
         if (blockIdx.x >= ctas) {
             if (t == 0) join->first = -1;
@@ -629,12 +635,13 @@ struct ka {
         }
         const uint32_t share = total / ctas, more = total - share * ctas; // the first `more` CTAs have one place more
         const uint32_t from = blockIdx.x * share + min(blockIdx.x, more), to = from + share + (blockIdx.x < more), x1 = tiles_of(from, to);
-        ka_item it = place(from);
+        uint32_t base;
+        ka_item it = place(from, base);
         if (t == 32) { // does an item begin in the CTA before and go on here?  (another warp than the copies')
             lb_kv4_join j;
             j.first = -1;
             if (x1 && it.tile > 0) {
-                const uint32_t begin = from - (uint32_t)it.tile, last = begin + (uint32_t)it.tiles - 1u; // places of its first and last tile
+                const uint32_t begin = base + KA_ITEM, last = begin + KA_STEP * (uint32_t)(it.tiles - 1); // where its first and its last tile begin
                 if (begin >= from - share - (blockIdx.x - 1 < more)) {
                     j.first = (int)blockIdx.x - 1;
                     j.last = (int)(last < more * (share + 1) ? last / (share + 1) : more + (last - more * (share + 1)) / share);
@@ -646,7 +653,7 @@ struct ka {
             }
             *join = j;
         }
-        if (!x1) return; // an item's first place alone
+        if (!x1) return; // an item's first places alone
         if (t == 0) {
             ka_item a = it;
             uint32_t i = 0;
