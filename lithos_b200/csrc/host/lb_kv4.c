@@ -97,13 +97,15 @@ LB_API int lb_kv4_attention(lb_ctx* c, const lb_kv4_cache* cache, const lb_kv4_b
     p.HQ = n_heads; p.type = type; p.rot_dims = rot_dims; p.eps = eps;
     p.wide = ((q | gate | (uint64_t)row_stride * (uint64_t)size_of(type) | (uint64_t)head_stride * (uint64_t)size_of(type)) & 15) == 0;
     p.out_wide = out % 16 == 0;
-    /* no more CTAs than full sequences have work for */
-    const int64_t most = (int64_t)batch->n_reqs * HKV * sets * ((cache->max_ctx + LB_KV4_TILE(D) - 1) / LB_KV4_TILE(D) + 2);
+    /* full sequences' items: places in the kernel's line of work, which it counts in 32 bits; no more CTAs than they have work for */
+    const int64_t items = (int64_t)batch->n_reqs * HKV * sets, tiles = (cache->max_ctx + LB_KV4_TILE(D) - 1) / LB_KV4_TILE(D);
+    if (items * (LB_KV4_STEP * tiles + LB_KV4_ITEM) > UINT32_MAX)
+        return lb_fail(c, LB_ERR_INVALID, "lb_kv4_attention: %d requests of up to %d rows, %d KV heads, %d columns: more work than a call can count", batch->n_reqs, cache->max_ctx, HKV, max_new * G);
+    const int64_t most = items * (tiles + LB_KV4_ITEM / LB_KV4_STEP + 1);
     int ctas = c->sm_count * LB_KV4_CTAS < LB_KV4_MAX_CTAS ? c->sm_count * LB_KV4_CTAS : LB_KV4_MAX_CTAS;
     if (ctas > most) ctas = (int)most;
     void* params[] = {&p, &ctas};
     LB_TRY(lb_launch(c, by_dim(D, LBK_kv4_attn_64, LBK_kv4_attn_128, LBK_kv4_attn_256), (unsigned)ctas, 1, 1, 256,
                      LB_KV4_SMEM, params, 1));
-    if (ctas == 1) return LB_OK; /* nothing is cut */
     return lb_launch(c, by_dim(D, LBK_kv4_merge_64, LBK_kv4_merge_128, LBK_kv4_merge_256), 2u * (unsigned)c->sm_count, 1, 1, 256, 0, params, 1);
 }

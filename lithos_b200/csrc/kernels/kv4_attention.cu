@@ -74,8 +74,8 @@ __device__ __forceinline__ int ka_exponent(uint32_t bits) { return max((int)(bit
 
 struct ka_item { int r, kv, z, tile, tiles; }; // a place in the line of tiles
 
-#define KA_STEP 2u // places of a tile in the line of work
-#define KA_ITEM 3u // and of an item's queries and results in front of its tiles
+#define KA_STEP ((uint32_t)LB_KV4_STEP)
+#define KA_ITEM ((uint32_t)LB_KV4_ITEM)
 #define KA_LIFT 4.f  // probabilities are 2^4 at their reference
 #define KA_OVER 6.f  // and may pass it by 2^6
 #define KA_WIDE 0x14001400u // a scale may pass its group's reference by 2^5: fp16 bits

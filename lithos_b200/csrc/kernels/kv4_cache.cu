@@ -145,7 +145,7 @@ __device__ __forceinline__ void kv4_append_body(const lb_kv4_rows_params& p) {
                 none = fmaf(v, 0.f, none); // a NaN if one of them is, or is infinite
                 hi = j == 0 || x[j] > hi ? x[j] : hi;
             }
-            if (size > 65504.f || none != 0.f) { // what fp16 holds: a value beyond it is cut off
+            if (size >= 65504.f || none != 0.f) { // what fp16 holds: a value beyond it is cut off
                 hi = -65504.0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {

@@ -603,6 +603,8 @@ typedef struct {
 /* The attention kernel: columns taken at a time, rows of a tile (36 KB), CTAs per SM and at most, ring stages.  Shared memory: the ring, probabilities, queries, the rest */
 #define LB_KV4_COLS 8
 #define LB_KV4_TILE(D) (32768 / (D))
+#define LB_KV4_STEP 2 /* places of a tile in the line of work */
+#define LB_KV4_ITEM 3 /* and of an item's queries and results in front of its tiles */
 #define LB_KV4_CTAS 2
 #define LB_KV4_MAX_CTAS 1024
 #define LB_KV4_STAGES 2

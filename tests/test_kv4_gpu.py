@@ -385,6 +385,9 @@ def test_refusals(lb, ctx):
     for rest in ((null, None, 0, 0, 1, None, b, 1), (b, None, 0, 0, 1, None, null, 1), (b, None, 0, 0, 1, None, b, 0), (b, None, 0, 0, 1, None, b, 17), (b, None, 0, 0, 1, None, b, 1, 0),
                  (b, None, 0, 0, 1, None, b, 1, 17), (b, None, 0, 60, 1, None, b, 1), (b, None, -8, 0, 1, None, b, 1), (b, at(2), 0, 0, 1, None, b, 1), (b, None, 0, 0, 1, None, at(1), 1)):
         bad(ctx.kv4_attention, *good, *rest)
+    # 256 requests that all read the longest cache with every column there is: 256 * 32 * 32 items of 2 * 8192 + 3 places pass 2^32
+    most = lb.Kv4Cache(cache[0], 1, 1 << 20, 32, 256), lb.Kv4Batch(b.ptr, b.ptr, b.ptr, 256, 256)
+    bad(ctx.kv4_attention, *most, b, None, 0, 0, 1, None, b, 512, 16)
     b.free()
 
 
