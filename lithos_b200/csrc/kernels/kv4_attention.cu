@@ -14,15 +14,15 @@
 //     16 rows, leaves p scale in shared memory as operands, and adds up a group's 64 features over its part of the tile.  References are standing: probabilities are
 //     taken against the largest score, and weights against the largest scale, at the last time that a score passed its reference by 2^6 or a scale by 2^5, for which
 //     fp16 has room; so a tile usually costs one barrier and no exchange of maxima.
-//   * All tiles of all items are dealt evenly to the CTAs in one line, with places for an item's start and end, so that ragged batches balance; an item cut by a border
-//     leaves records that kv4_merge joins in order.
+//   * All tiles of all items are dealt evenly to the CTAs in one line, with places of one and a half tiles for an item's queries and results, so that ragged batches balance (32
+//     sequences: 74 us without such places, 61 with a tile's, 57 so); an item cut by a border leaves records that kv4_merge joins in order.
 // mma.sync rather than tcgen05: the columns are few (6 for one token of 24 heads on 4), and codes would have to be widened into shared or tensor memory for it.
 // Bound by three things at once: per tile and SM, some 800 instructions a warp (issue slots 50 - 60 % busy), 200 passes through shared memory a warp (two thirds of its time: queries 64,
 // copies in 36, codes 32, weights out and in 32, scales 36) and the tensor pipe (35 - 40 %); what overlaps them is 16 warps an SM, as many as 128 registers leave.
-// us a call with the merge, 24 / 4 heads of 256: one sequence of 4096 rows 12.5, of 100 001 48.4 (2.4 TB/s); 32 of 40 to 16 000 rows 74 (1.9 TB/s); 16 of 500 to 9001 rows with up to 5
-// new tokens 87; 64 of 17 to 3001 rows, 32 / 8 heads of 128: 50.  Not so: warps of their own for scores and read-outs (8 + 8 with the queries in registers 66 us at
+// us a call with the merge, 24 / 4 heads of 256: one sequence of 4096 rows 12.4, of 100 001 46.6 (2.5 TB/s); 32 of 40 to 16 000 rows 57 (2.5 TB/s); 16 of 500 to 9001 rows with up to 5
+// new tokens 83; 64 of 17 to 3001 rows, 32 / 8 heads of 128: 40.6.  Not so: warps of their own for scores and read-outs (8 + 8 with the queries in registers 66 us at
 // 100 001 rows, two CTAs of 6 + 2 60); 16 columns at a time on half as many warps (150 where passes of eight took 118); three CTAs of four warps with the queries in
-// registers (54); maxima exchanged for every tile (52).
+// registers (54); maxima exchanged for every tile (52); the next launch let in early (13.9 at 4096 rows: its waiting CTAs are in the way).
 #include "kv4.cuh"
 
 #define KA_WARPS 8
