@@ -331,14 +331,15 @@ struct ka {
         }
     }
 
-    // one tile; false: the wait for it gave up
+    // one tile; false: the wait for it gave up.  FULL: all of its rows are there and every column sees them
+    template <bool FULL>
     __device__ __forceinline__ bool tile(const ka_item& it, uint32_t i_tile, uint32_t tiles) {
-        const int slot = i_tile % NS, nb = min(BLOCKS, (len - it.tile * TILE + 15) >> 4), base = it.tile * TILE + 16 * warp;
-        const bool edge = base + 128 * (BW - 1) + 15 > first_new; // rows that not every column sees, or that are not there
+        const int slot = i_tile % NS, nb = FULL ? BLOCKS : min(BLOCKS, (len - it.tile * TILE + 15) >> 4), base = it.tile * TILE + 16 * warp;
+        const bool edge = !FULL && base + 128 * (BW - 1) + 15 > first_new; // rows that not every column sees, or that are not there
         const unsigned char* ring = s.ring[slot];
         rows r[BW];
         bool landed = mbar_wait(&s.full[slot], (i_tile / NS) & 1), over = !landed;
-        if (warp < nb && landed) {
+        if (FULL || (warp < nb && landed)) {
             float a[BW][S][2][4];
             uint2 w[BW][S][2];
             uint32_t pair[BW][2];
@@ -414,12 +415,12 @@ struct ka {
             }
         }
         if (i_tile) landed = mbar_wait(&s.pfree, (i_tile - 1) & 1) && landed; // the tile before has been read out
-        if (warp < nb)
+        if (FULL || warp < nb)
 #pragma unroll
             for (int k = 0; k < BW; ++k) weigh(r[k], warp + 8 * k, edge, base + 128 * k + 4 * ft);
         if (__syncthreads_or(over || !landed)) {
             if (__syncthreads_or(!landed)) return false;
-            renew(r, warp < nb, edge, base + 4 * ft);
+            renew(r, FULL || warp < nb, edge, base + 4 * ft);
         }
         uint32_t lv[BW][2]; // p lowest and the sum of p: lowest values as an operand, ones in its fifth column
 #pragma unroll
@@ -433,12 +434,12 @@ struct ka {
             lv[k][1] = g == 4 ? 0x3c003c00u : __byte_perm(vr.z, vr.w, 0x7632);
         }
         const int group = warp % S, part = warp / S;
-        if (part < nb) {
+        if (FULL || part < nb) {
             float d[8][4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int b = k * PARTS + part;
-                if (k && b >= nb) break;
+                if (!FULL && k && b >= nb) break;
                 const uint4 v = *reinterpret_cast<const uint4*>(ring + b * BLK + 8 * D + group * 512 + lane * 16);
                 const uint32_t a0 = __byte_perm(v.x, v.y, 0x5410), a1 = __byte_perm(v.x, v.y, 0x7632), c0 = __byte_perm(v.z, v.w, 0x5410), c1 = __byte_perm(v.z, v.w, 0x7632);
                 const uint4 pa = s.p[group][b][lane];
@@ -673,7 +674,7 @@ struct ka {
                 __syncthreads();
                 f = s.factor[g];
             }
-            if (!tile(it, x, x1)) { // a copy never landed: say so, let the others land, leave
+            if (!(it.tile * TILE + TILE - 1 <= first_new ? tile<true>(it, x, x1) : tile<false>(it, x, x1))) { // a copy never landed: say so, let the others land, leave
                 if (t == 0) {
                     atomicExch(p.b.status, KV_FAIL_FULL);
                     for (uint32_t y = x; y < s.requested; ++y) mbar_wait(&s.full[y % NS], (y / NS) & 1);
