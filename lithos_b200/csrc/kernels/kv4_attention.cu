@@ -84,14 +84,14 @@ template <int D>
 struct ka {
     static constexpr int S = D / 64, PARTS = KA_WARPS / S, BLK = LB_KV4_BLOCK(D), NS = LB_KV4_STAGES;
     static constexpr int BW = 4 / S, TILE = LB_KV4_TILE(D), BLOCKS = TILE / 16; // blocks of a warp; block w + 8 k is warp w's
+    static constexpr int P_BUFS = D == 64 ? 1 : 2; // what there is room for
     struct alignas(128) smem {
         unsigned char ring[NS][BLOCKS * BLK];
-        uint4 p[S][BLOCKS][32];         // p scale as operands of the products: [group][block of the tile]; an item's sums at its end
+        uint4 p[P_BUFS][BLOCKS][32];    // probabilities in two terms, a block's as a lane has them; an item's sums at its end
         uint4 q[4 * S][32];             // queries likewise: step 4 group + 2 word + u
         uint2 qsum[32];                 // sums of a query's groups as the operand that meets (scale, lowest)
         float part[KA_WARPS][KA_COLS][S + 1];
         alignas(16) float max[KA_COLS][KA_WARPS];
-        alignas(16) uint2 scale[KA_WARPS];
         double freq[D / 2];
         float factor[KA_COLS], m[KA_COLS], l[KA_COLS], low[KA_COLS][S];
         uint64_t full[NS], pfree;
@@ -270,9 +270,9 @@ struct ka {
     float m;            // reference of column g's scores, in log2 units
     float low[4];       // of this warp's rows, column g in two terms: sums of p lowest of groups 2 ft, 2 ft + 1; ft = 2: the sum of p
     float acc[8][2];    // of this warp's group and part, column g: features 8 (2 ft, 2 ft + 1) + j: of a for even j, of a + 16 b for odd ones
-    uint32_t ref[S];    // fp16 bits, twice, of the scales that the groups' are taken against
-    uint32_t room[S];   // and of the largest that they may take
-    uint32_t up[S];     // fp16 2^-1 over a reference's power of two, twice
+    uint32_t ref;       // fp16 bits, twice, of the scale that this warp's are taken against
+    uint32_t room;      // and of the largest that they may be
+    uint32_t up;        // fp16 2^-1 over the reference's power of two, twice
     float f;            // of column g's scores
     int len, first_new; // rows of the item, the first of its new ones
 
@@ -283,8 +283,7 @@ struct ka {
         low[0] = low[1] = low[2] = low[3] = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = 0.f;
-#pragma unroll
-        for (int q = 0; q < S; ++q) ref[q] = room[q] = up[q] = 0u;
+        ref = room = up = 0u;
     }
 
     // (scale, lowest) of four rows, of those that are there
@@ -292,50 +291,43 @@ struct ka {
         return make_uint4(row0 < len ? v.x : 0u, row0 + 1 < len ? v.y : 0u, row0 + 2 < len ? v.z : 0u, row0 + 3 < len ? v.w : 0u);
     }
     static __device__ __forceinline__ uint32_t lowest_or_0(uint32_t pair) { return (pair & 0x7fff0000u) < 0x7c000000u ? pair : 0u; }
-    // a thread's scores of a block of 16 rows: rows row0 .. row0 + 3, column g; the values' scales of these rows as fp16 pairs
+    // a thread's scores of a block of 16 rows: rows 4 ft .. 4 ft + 3, column g; probabilities in two terms
     struct rows {
         float sc[4];
-        uint32_t s01[S], s23[S];
-        uint2 hi, lo; // probabilities in two terms
+        uint2 hi, lo;
     };
-    // the largest scale of a group over these rows, in the halves of a word; a NaN has no say: columns before its row are not to notice it
-    static __device__ __forceinline__ uint32_t widest(uint32_t s01, uint32_t s23, bool edge) {
-        if (edge) {
-            s01 &= __vcmpltu2(s01, 0x7c007c00u);
-            s23 &= __vcmpltu2(s23, 0x7c007c00u);
-        }
-        return __vmaxu2(s01, s23);
-    }
 
-    // scores -> probabilities, p scale in shared memory
-    __device__ __forceinline__ void weigh(rows& r, int b, bool edge, int row0) {
+    // scores -> probabilities, for whoever reads the block out
+    __device__ __forceinline__ void weigh(rows& r, uint4* to) {
         const float less = KA_LIFT - (m == -INFINITY ? 0.f : m); // a column that has seen nothing yet
         float pr[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) pr[i] = ka_exp2(fmaf(r.sc[i], f, less));
         ka_split(pr[0], pr[1], r.hi.x, r.lo.x);
         ka_split(pr[2], pr[3], r.hi.y, r.lo.y);
-        uint32_t on01 = ~0u, on23 = ~0u;
-        if (edge) { // a NaN's group reaches the columns that see its row, and no other as 0 times NaN
-            const int lim = s.limit[g];
-            on01 = (row0 <= lim ? 0xffffu : 0u) | (row0 + 1 <= lim ? 0xffff0000u : 0u);
-            on23 = (row0 + 2 <= lim ? 0xffffu : 0u) | (row0 + 3 <= lim ? 0xffff0000u : 0u);
-        }
+        to[lane] = make_uint4(r.hi.x, r.lo.x, r.hi.y, r.lo.y);
+    }
+    // a new reference for the scales of this warp's group
+    __device__ __forceinline__ void widen(uint32_t v) {
+        v = __vmaxu2(v, __shfl_xor_sync(0xffffffffu, v, 1));
+        v = __vmaxu2(v, __shfl_xor_sync(0xffffffffu, v, 2));
+        v = max(v & 0xffffu, v >> 16);
+        const int before = ka_exponent(ref & 0xffffu);
+        ref = max(ref & 0xffffu, v) * 0x10001u;
+        room = ref ? __vaddus2(ref, KA_WIDE) : 0u;
+        const int e = ka_exponent(ref & 0xffffu);
+        const float shrink = ka_pow2(before - e);
+        const __half2 u = __float2half2_rn(ka_pow2(-1 - e));
+        up = *reinterpret_cast<const uint32_t*>(&u);
 #pragma unroll
-        for (int q = 0; q < S; ++q) {
-            // (hi + lo) scale in two terms: the first product rounded, what the rounding left exactly, and lo scale on top of that
-            uint4 o;
-            ka_scale(r.hi.x, r.lo.x, edge ? r.s01[q] & on01 : r.s01[q], up[q], o.x, o.y);
-            ka_scale(r.hi.y, r.lo.y, edge ? r.s23[q] & on23 : r.s23[q], up[q], o.z, o.w);
-            s.p[q][b][lane] = o;
-        }
+        for (int j = 0; j < 8; ++j) { acc[j][0] *= shrink; acc[j][1] *= shrink; }
     }
 
     // one tile; false: the wait for it gave up.  FULL: all of its rows are there and every column sees them
     template <bool FULL>
     __device__ __forceinline__ bool tile(const ka_item& it, uint32_t i_tile, uint32_t tiles) {
-        const int slot = i_tile % NS, nb = FULL ? BLOCKS : min(BLOCKS, (len - it.tile * TILE + 15) >> 4), base = it.tile * TILE + 16 * warp;
-        const bool edge = !FULL && base + 128 * (BW - 1) + 15 > first_new; // rows that not every column sees, or that are not there
+        const int slot = i_tile % NS, nb = FULL ? BLOCKS : min(BLOCKS, (len - it.tile * TILE + 15) >> 4), row0 = it.tile * TILE + 4 * ft, group = warp % S, part = warp / S;
+        uint4 (*const pw)[32] = s.p[P_BUFS == 2 ? i_tile & 1 : 0];
         const unsigned char* ring = s.ring[slot];
         rows r[BW];
         bool landed = mbar_wait(&s.full[slot], (i_tile / NS) & 1), over = !landed;
@@ -371,7 +363,6 @@ struct ka {
 #pragma unroll
             for (int k = 0; k < BW; ++k) {
                 const unsigned char* blk = ring + (warp + 8 * k) * BLK;
-                const int row0 = base + 128 * k + 4 * ft;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) { // lowest sum(q)
                     float d[4];
@@ -387,21 +378,11 @@ struct ka {
                     r[k].sc[2] = fmaf(ka_pair(pr.z).x, a[k][q][1][0] + a[k][q][1][2], r[k].sc[2]);
                     r[k].sc[3] = fmaf(ka_pair(pr.w).x, a[k][q][1][1] + a[k][q][1][3], r[k].sc[3]);
                 }
-#pragma unroll
-                for (int q = 0; q < S; ++q) {
-                    uint4 vr = *reinterpret_cast<const uint4*>(blk + 17 * D + (q * 16 + 4 * ft) * 4);
-                    if (edge) vr = there(vr, row0, len);
-                    r[k].s01[q] = __byte_perm(vr.x, vr.y, 0x5410);
-                    r[k].s23[q] = __byte_perm(vr.z, vr.w, 0x5410);
-                    // does something pass its reference by more than there is room for?  A reference of 0 has none
-                    const uint32_t v = widest(r[k].s01[q], r[k].s23[q], edge);
-                    over |= v != __vminu2(v, room[q]);
-                }
-                if (edge) {
-                    const int lim = s.limit[g];
+                if (!FULL) { // rows that the column does not see, or that are not there
+                    const int lim = s.limit[g] - row0 - 16 * (warp + 8 * k);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (row0 + i > lim) r[k].sc[i] = -INFINITY;
+                        if (i > lim) r[k].sc[i] = -INFINITY;
                 }
                 over |= fmaf(fmaxf(fmaxf(r[k].sc[0], r[k].sc[1]), fmaxf(r[k].sc[2], r[k].sc[3])), f, -m) > KA_OVER;
             }
@@ -409,31 +390,52 @@ struct ka {
 #pragma unroll
             for (int k = 0; k < BW; ++k) {
                 r[k].sc[0] = r[k].sc[1] = r[k].sc[2] = r[k].sc[3] = -INFINITY;
-#pragma unroll
-                for (int q = 0; q < S; ++q) r[k].s01[q] = r[k].s23[q] = 0u;
                 r[k].hi = r[k].lo = make_uint2(0u, 0u);
             }
         }
-        if (i_tile) landed = mbar_wait(&s.pfree, (i_tile - 1) & 1) && landed; // the tile before has been read out
+        // the tile before has been read out; with two buffers the one before that, which everybody had done at the tile before's barrier
+        if (P_BUFS == 1 && i_tile) landed = mbar_wait(&s.pfree, (i_tile - 1) & 1) && landed;
         if (FULL || warp < nb)
 #pragma unroll
-            for (int k = 0; k < BW; ++k) weigh(r[k], warp + 8 * k, edge, base + 128 * k + 4 * ft);
+            for (int k = 0; k < BW; ++k) weigh(r[k], pw[warp + 8 * k]);
+        // the values' scales of the blocks that this warp reads out
+        uint32_t s01[4], s23[4], wide = 0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int b = k * PARTS + part;
+            s01[k] = s23[k] = 0u;
+            if (!FULL && b >= nb) continue;
+            uint4 v = *reinterpret_cast<const uint4*>(ring + b * BLK + 17 * D + (group * 16 + 4 * ft) * 4);
+            if (!FULL) v = there(v, row0 + 16 * b, len);
+            s01[k] = __byte_perm(v.x, v.y, 0x5410);
+            s23[k] = __byte_perm(v.z, v.w, 0x5410);
+            if (FULL) wide = __vmaxu2(wide, __vmaxu2(s01[k], s23[k]));
+            else { // a NaN has no say here: columns before its row are not to notice it
+                wide = __vmaxu2(wide, s01[k] & __vcmpltu2(s01[k], 0x7c007c00u));
+                wide = __vmaxu2(wide, s23[k] & __vcmpltu2(s23[k], 0x7c007c00u));
+            }
+            if (!FULL) { // a NaN's group reaches the columns that see its row, and no other as 0 times NaN
+                const int lim = s.limit[g] - row0 - 16 * b;
+                s01[k] &= (lim >= 0 ? 0xffffu : 0u) | (lim >= 1 ? 0xffff0000u : 0u);
+                s23[k] &= (lim >= 2 ? 0xffffu : 0u) | (lim >= 3 ? 0xffff0000u : 0u);
+            }
+        }
+        if (__any_sync(0xffffffffu, wide != __vminu2(wide, room))) widen(wide); // a reference of 0 has no room
         if (__syncthreads_or(over || !landed)) {
             if (__syncthreads_or(!landed)) return false;
-            renew(r, FULL || warp < nb, edge, base + 4 * ft);
+            renew(r, FULL || warp < nb, pw);
         }
         uint32_t lv[BW][2]; // p lowest and the sum of p: lowest values as an operand, ones in its fifth column
 #pragma unroll
         for (int k = 0; k < BW; ++k) {
             uint4 vr = *reinterpret_cast<const uint4*>(ring + (warp + 8 * k) * BLK + 17 * D + ((g % S) * 16 + 4 * ft) * 4);
-            if (edge) { // blocks that are not there, too; where a column sees a NaN's row, p scale is NaN
-                vr = there(vr, base + 128 * k + 4 * ft, len);
+            if (!FULL) { // blocks that are not there, too; where a column sees a NaN's row, p scale is NaN
+                vr = there(vr, row0 + 16 * (warp + 8 * k), len);
                 vr.x = lowest_or_0(vr.x); vr.y = lowest_or_0(vr.y); vr.z = lowest_or_0(vr.z); vr.w = lowest_or_0(vr.w);
             }
             lv[k][0] = g == 4 ? 0x3c003c00u : __byte_perm(vr.x, vr.y, 0x7632);
             lv[k][1] = g == 4 ? 0x3c003c00u : __byte_perm(vr.z, vr.w, 0x7632);
         }
-        const int group = warp % S, part = warp / S;
         if (FULL || part < nb) {
             float d[8][4];
 #pragma unroll
@@ -442,7 +444,11 @@ struct ka {
                 if (!FULL && k && b >= nb) break;
                 const uint4 v = *reinterpret_cast<const uint4*>(ring + b * BLK + 8 * D + group * 512 + lane * 16);
                 const uint32_t a0 = __byte_perm(v.x, v.y, 0x5410), a1 = __byte_perm(v.x, v.y, 0x7632), c0 = __byte_perm(v.z, v.w, 0x5410), c1 = __byte_perm(v.z, v.w, 0x7632);
-                const uint4 pa = s.p[group][b][lane];
+                // (hi + lo) scale in two terms: the first product rounded, what the rounding left exactly, and lo scale on top of that
+                const uint4 pk = pw[b][lane];
+                uint4 pa;
+                ka_scale(pk.x, pk.y, s01[k], up, pa.x, pa.y);
+                ka_scale(pk.z, pk.w, s23[k], up, pa.z, pa.w);
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const uint32_t y = j < 4 ? a0 : a1, z = j < 4 ? c0 : c1;
@@ -484,59 +490,25 @@ struct ka {
     }
 
     // new references: the exchange of maxima, and the probabilities again
-    __device__ __forceinline__ void renew(rows (&r)[BW], bool live, bool edge, int row0) {
+    __device__ __forceinline__ void renew(rows (&r)[BW], bool live, uint4 (*pw)[32]) {
         float best = -INFINITY;
-        uint2 mx = make_uint2(0u, 0u); // the groups' largest scales, 16 bits each
 #pragma unroll
         for (int k = 0; k < BW; ++k) best = fmaxf(best, fmaxf(fmaxf(r[k].sc[0], r[k].sc[1]), fmaxf(r[k].sc[2], r[k].sc[3])));
-#pragma unroll
-        for (int q = 0; q < S; ++q) {
-            uint32_t v = 0u;
-#pragma unroll
-            for (int k = 0; k < BW; ++k) v = __vmaxu2(v, widest(r[k].s01[q], r[k].s23[q], edge));
-            v = max(v & 0xffffu, v >> 16) << (16 * (q & 1));
-            if (q & 2) mx.y |= v;
-            else mx.x |= v;
-        }
         best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
         best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
         if (ft == 0) s.max[g][warp] = best;
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            mx.x = __vmaxu2(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o));
-            if (S > 2) mx.y = __vmaxu2(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o));
-        }
-        if (lane == 0) s.scale[warp] = mx;
         __syncthreads();
         const float4 a = *reinterpret_cast<const float4*>(s.max[g]), b = *reinterpret_cast<const float4*>(s.max[g] + 4);
         const float now = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))) * f, top = fmaxf(m, now);
         const float corr = top == -INFINITY ? 0.f : ka_exp2(m - top);
         m = top;
-        mx = make_uint2(0u, 0u);
-#pragma unroll
-        for (int w = 0; w < KA_WARPS; w += 2) {
-            const uint4 v = *reinterpret_cast<const uint4*>(&s.scale[w]);
-            mx.x = __vmaxu2(mx.x, __vmaxu2(v.x, v.z));
-            mx.y = __vmaxu2(mx.y, __vmaxu2(v.y, v.w));
-        }
-        float shrink = corr;
-#pragma unroll
-        for (int q = 0; q < S; ++q) {
-            const uint32_t v = __byte_perm(q & 2 ? mx.y : mx.x, 0u, q & 1 ? 0x3232 : 0x1010), old = ref[q];
-            ref[q] = __vmaxu2(old, v);
-            room[q] = ref[q] ? __vaddus2(ref[q], KA_WIDE) : 0u;
-            const int e = ka_exponent(ref[q] & 0xffffu);
-            if (q == warp % S) shrink = corr * ka_pow2(ka_exponent(old & 0xffffu) - e);
-            const __half2 u = __float2half2_rn(ka_pow2(-1 - e));
-            up[q] = *reinterpret_cast<const uint32_t*>(&u);
-        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) low[i] *= corr;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { acc[j][0] *= shrink; acc[j][1] *= shrink; }
+        for (int j = 0; j < 8; ++j) { acc[j][0] *= corr; acc[j][1] *= corr; }
         if (live)
 #pragma unroll
-            for (int k = 0; k < BW; ++k) weigh(r[k], warp + 8 * k, edge, row0 + 128 * k);
+            for (int k = 0; k < BW; ++k) weigh(r[k], pw[warp + 8 * k]);
         __syncthreads();
     }
 
@@ -575,10 +547,7 @@ struct ka {
         if (2 * ft + 1 < S) s.part[warp][g][2 * ft + 1] = low[1] + low[3];
         if (ft == 2) s.part[warp][g][S] = low[0] + low[2];
         if (ft == 0 && warp == 0) s.m[g] = m;
-        int e = 0;
-#pragma unroll
-        for (int q = 0; q < S; ++q)
-            if (q == group) e = ka_exponent(ref[q] & 0xffffu);
+        const int e = ka_exponent(ref & 0xffffu);
         const float even = ka_pow2(e + 25), odd = even * 0.0625f; // 2^24 over 2^(-1 - e)
         for (int turn = 0; turn < PARTS; ++turn) { // the parts of a tile one after the other
             __syncthreads();
