@@ -306,7 +306,8 @@ int lb_kv4_append(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* ba
                   int rot_dims, float rope_theta, float eps);
 /* The rows that the batch names, as values: k_out, v_out [rows, kv_heads, dim] of element type `type` (one rounding) */
 int lb_kv4_read(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t k_out, uint64_t v_out, int type);
-/* Attention of the batch's new tokens, whose rows are in the cache: token i of request r sees rows 0 .. pos[r] + i.
+/* Attention of the batch's new tokens, whose rows are in the cache: token i of request r sees rows 0 .. pos[r] + i.  Several requests
+ * may read the same sequence.
  * q and gate (0: none): element type `type`, head h of token row j at j * row_stride + h * head_stride elements (row_stride 0: n_heads * head_stride, head_stride 0: dim); q is
  * normalised per head (q_norm_w; 0: not) and rotated like the keys, and goes in with 22 bits; the result is multiplied by sigmoid(gate).  n_heads: 1 to 16 times
  * kv_heads.  max_new: the most tokens a request of the batch has, 1 .. LB_KV4_MAX_NEW.  out fp16 [rows, n_heads, dim], what lb_gemm_int4 takes; it

@@ -422,3 +422,58 @@ def test_captured_graph_takes_new_positions(lb, ctx):
     assert np.array_equal(eager[0], replayed[0]) and np.array_equal(eager[1], replayed[1])
     graph.destroy()
     case.free()
+
+
+@pytest.mark.parametrize("dim,new", [(64, 1), (128, 5), (256, 1), (256, 5)])
+@pytest.mark.parametrize("way", ["up", "down", "mixed"])
+def test_attention_scales_by_block(lb, ctx, dim, new, way):
+    """every block of 16 rows and every group has its own order of magnitude: the scales that warps take theirs against differ, and move at different tiles"""
+    S, blocks = dim // 64, 128
+    case = kc.Case(ctx, dim, 2, 1, 16 * blocks, seqs=[0], pos=[16 * blocks - 20], new=[new])
+    raw = case.cache[0, :, :, 16 * dim:].copy().view(np.float16).reshape(2, blocks, 2, S, 16, 2)
+    rng = np.random.default_rng(21)
+    power = {"up": np.linspace(-4, 3, blocks)[:, None] + np.zeros(S), "down": np.linspace(3, -4, blocks)[:, None] + np.zeros(S), "mixed": rng.uniform(-4, 3, (blocks, S))}[way]
+    raw[:, :, 1] = (raw[:, :, 1] * (10.0 ** power)[None, :, :, None, None]).astype(np.float16)
+    case.cache[0, :, :, 16 * dim:] = raw.reshape(2, blocks, -1).view(np.uint8)
+    case.d_cache.upload(case.cache)
+    attention(lb, ctx, case, 3, lb.IN_F32)
+    case.free()
+
+
+def test_attention_requests_of_one_sequence(lb, ctx):
+    """several requests may read the same sequence, each up to its own place"""
+    case = kc.Case(ctx, 128, 2, 2, 1024, seqs=[1, 1, 0, 1], pos=[900, 3, 500, 900], new=[2, 1, 1, 2])
+    attention(lb, ctx, case, 4, lb.IN_F32)
+    case.free()
+
+
+def test_two_graphs_in_turn(lb, ctx):
+    """graphs of different shapes share the context's workspace: replayed in turn and twice in a row, the same as the calls"""
+    rng = np.random.default_rng(4)
+    cases = [kc.Case(ctx, 256, 2, 3, 2048, seqs=[2, 0, 1], pos=[2000, 5, 700], new=[2, 1, 3]), kc.Case(ctx, 64, 4, 2, 4096, seqs=[1, 0], pos=[4000, 100], new=[1, 1])]
+    steps, graphs, outs, want = [], [], [], []
+    for case, G in zip(cases, (3, 2)):
+        d_q = ctx.to_device(rng.standard_normal((case.rows, case.heads * G * case.dim)).astype(np.float32))
+        out = ctx.alloc(case.rows * case.heads * G * case.dim * 2)
+        steps.append((case, d_q, out, case.heads * G))
+        outs.append(out)
+
+    def run(case, d_q, out, heads):
+        ctx.kv4_attention(case.desc, case.batch, d_q, None, 0, 0, lb.IN_F32, None, out, heads, max(case.new), 64, THETA, EPS)
+    for step in steps:
+        run(*step)
+        want.append(step[2].download(np.float16).copy())
+        ctx.begin_capture()
+        run(*step)
+        graphs.append(ctx.end_capture())
+    for order in ((0, 1, 0, 1), (1, 1, 0, 0)):
+        for out in outs:
+            out.upload(np.zeros(out.nbytes // 2, np.float16))
+        for g in order:
+            graphs[g].launch()
+        for out, w in zip(outs, want):
+            assert np.array_equal(out.download(np.float16), w)
+    for g in graphs:
+        g.destroy()
+    for case, d_q, out, _ in steps:
+        d_q.free(), out.free(), case.free()
