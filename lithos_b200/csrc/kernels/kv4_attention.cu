@@ -21,8 +21,8 @@
 // mma.sync rather than tcgen05: the columns are few (6 for one token of 24 heads on 4), and codes would have to be widened into shared or tensor memory for it.
 // Bound by the latency of a tile's steps, with 16 warps an SM (as many as 128 registers leave) to hide it: per tile and SM some 610 instructions a warp (issue slots 44 %
 // busy), 180 passes through shared memory a warp (half of its time: queries 64, codes 32, copies in 36, scales 36, probabilities 20), the tensor pipe 38 %.
-// us a call with the merge, 24 / 4 heads of 256: one sequence of 4096 rows 11.2, of 100 001 41.0 (2.8 TB/s); 32 of 40 to 16 000 rows 51.7 (2.8 TB/s); 16 of 500 to 9001 rows with up
-// to 5 new tokens 72.4; 64 of 17 to 3001 rows, 32 / 8 heads of 128: 38.9.  Tried without gain, us at 100 001 rows where 41 now or as given: warps of their own for scores and
+// us a call with the merge, 24 / 4 heads of 256: one sequence of 4096 rows 11.1, of 100 001 41.3 (2.8 TB/s); 32 of 40 to 16 000 rows 52 (2.8 TB/s); 16 of 500 to 9001 rows with up
+// to 5 new tokens 73.8; 64 of 17 to 3001 rows, 32 / 8 heads of 128: 37.3 (39.5 where the parts of a tile were added up in turns at an item's end).  Tried without gain, us at 100 001 rows where 41 now or as given: warps of their own for scores and
 // read-outs (8 + 8 with the queries in registers 66, two CTAs of 6 + 2 60, both where 48); 16 columns at a time on half as many warps (150 where passes of eight took 118); three CTAs of
 // four warps with the queries in registers (54 where 48); maxima exchanged for every tile (52 where 48); barriers and references of the warps that share blocks alone (41.5);
 // a block's scales by shuffles (41.3); the next launch let in early (13.9 at 4096 rows where 12.4: its waiting CTAs are in the way).
@@ -90,7 +90,10 @@ struct ka {
     static constexpr int P_BUFS = D == 64 ? 1 : 2; // what there is room for
     struct alignas(128) smem {
         unsigned char ring[NS][BLOCKS * BLK];
-        uint4 p[P_BUFS][BLOCKS][32];    // probabilities in two terms, a block's as a lane has them; an item's sums at its end
+        union {
+            uint4 p[P_BUFS][BLOCKS][32];        // probabilities in two terms, a block's as a lane has them
+            float sum[PARTS][KA_COLS][D + 4];   // at an item's end
+        };
         uint4 q[4 * S][32];             // queries likewise: step 4 group + 2 word + u
         uint2 qsum[32];                 // sums of a query's groups as the operand that meets (scale, lowest)
         float part[KA_WARPS][KA_COLS][S + 1];
@@ -544,7 +547,6 @@ struct ka {
     }
     // The item's columns, whole or this CTA's share of them.  `first`: the item's first tile was this CTA's, `last`: its last
     __device__ __forceinline__ void finish(const ka_item& it, bool first, bool last) {
-        float* sum = reinterpret_cast<float*>(&s.p[0][0][0]); // [KA_COLS][D]
         const int group = warp % S, part = warp / S, cols = min(KA_COLS, s.n[it.r] * G - it.z * KA_COLS);
         if (2 * ft < S) s.part[warp][g][2 * ft] = low[0] + low[2];
         if (2 * ft + 1 < S) s.part[warp][g][2 * ft + 1] = low[1] + low[3];
@@ -552,22 +554,13 @@ struct ka {
         if (ft == 0 && warp == 0) s.m[g] = m;
         const int e = ka_exponent(ref & 0xffffu);
         const float even = ka_pow2(e + 25), odd = even * 0.0625f; // 2^24 over 2^(-1 - e)
-        for (int turn = 0; turn < PARTS; ++turn) { // the parts of a tile one after the other
-            __syncthreads();
-            if (part == turn)
+        __syncthreads(); // the probabilities have been read
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < 8; j += 4) {
-                        float4* x = reinterpret_cast<float4*>(sum + g * D + group * 64 + 8 * (2 * ft + i) + j);
-                        float4 y = make_float4(acc[j][i] * even, (acc[j + 1][i] - acc[j][i]) * odd, acc[j + 2][i] * even, (acc[j + 3][i] - acc[j + 2][i]) * odd);
-                        if (turn) {
-                            const float4 w = *x;
-                            y.x += w.x; y.y += w.y; y.z += w.z; y.w += w.w;
-                        }
-                        *x = y;
-                    }
-        }
+            for (int j = 0; j < 8; j += 4)
+                *reinterpret_cast<float4*>(&s.sum[part][g][group * 64 + 8 * (2 * ft + i) + j]) =
+                    make_float4(acc[j][i] * even, (acc[j + 1][i] - acc[j][i]) * odd, acc[j + 2][i] * even, (acc[j + 3][i] - acc[j + 2][i]) * odd);
         __syncthreads();
         float* rec = p.records + ((size_t)blockIdx.x * 2 + (first ? 1 : 0)) * KA_COLS * LB_KV4_REC(D);
         for (int o = t; o < KA_COLS * D / 8; o += KA_THREADS) { // eight features a thread
@@ -580,7 +573,15 @@ struct ka {
                 l += s.part[w][c][S];
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = sum[c * D + f + j] + lo;
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
+#pragma unroll
+            for (int q = 0; q < PARTS; ++q) { // the parts of a tile in their order
+                const float4 a = *reinterpret_cast<const float4*>(&s.sum[q][c][f]), b = *reinterpret_cast<const float4*>(&s.sum[q][c][f + 4]);
+                v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+                v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += lo;
             put(it, first && last, rec, c, f, v, 1.f / l);
             if (!(first && last) && f == 0) {
                 rec[c * LB_KV4_REC(D) + D] = s.m[c];

@@ -608,7 +608,7 @@ typedef struct {
 #define LB_KV4_CTAS 2
 #define LB_KV4_MAX_CTAS 1024
 #define LB_KV4_STAGES 2
-#define LB_KV4_SMEM (LB_KV4_STAGES * 36864 + 16384 + 8192 + 9 * 1024)
+#define LB_KV4_SMEM (LB_KV4_STAGES * 36864 + 17408 + 8192 + 9 * 1024)
 
 /* ---- drafted tokens against the target's probabilities (verify.cu) -------------------------------------------- */
 #define LB_VD_REQS 256
