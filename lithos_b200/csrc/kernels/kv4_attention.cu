@@ -11,10 +11,11 @@
 //     by themselves (the products' own additions cut off); the output is fp16, what lb_gemm_int4 takes.
 //   * lowest_t sum(q) is one product more per 8 rows, p_t lowest_t and the sum of p one per 16.
 //   * A tile is 32768 / D rows, 36 KB, one bulk copy, requested by whichever warp is the last to be done with the place it goes to.  A warp does the scores of 256 / D blocks of
-//     16 rows and leaves their probabilities in shared memory; after a barrier it reads a group's 64 features out over its part of the tile, probabilities times that group's
-//     scales as operands (44.4 us at 100 001 rows with the products written for all groups by whoever has the scores, 41 so).  References are standing: probabilities are
-//     taken against the largest score, and a warp's weights against the largest scale, at the last time that a score passed its reference by 2^6 or a scale by 2^5, for
-//     which fp16 has room; so a tile usually costs one barrier and no exchange of maxima.  Tiles whose rows are all there and seen by every column, most, take a path
+//     16 rows and leaves their probabilities in shared memory; after a barrier it reads a group's 64 features out over its part of the tile, weights - probabilities times that
+//     group's scales, multiplied in 32 bits - as operands (44.4 us at 100 001 rows with the products written for all groups by whoever has the scores, 41 so).  References are standing:
+//     probabilities are taken against the largest score, and a warp's weights of a column against the largest of them, at the last time that one passed its reference by 2^6, for
+//     which fp16 has room; so a tile usually costs one barrier and no exchange of maxima.  (A reference from the scales alone, 2 % faster, lost the bits of all rows
+//     that have weight where a row that has none is of large scale.)  Tiles whose rows are all there and seen by every column, most, take a path
 //     without those checks (46.6 -> 44.4).
 //   * All tiles of all items are dealt evenly to the CTAs in one line, with places of one and a half tiles for an item's queries and results, so that ragged batches balance (32
 //     sequences: 74 us without such places, 61 with a tile's, 57 so); an item cut by a border leaves records that kv4_merge joins in order.
@@ -66,14 +67,6 @@ __device__ __forceinline__ void ka_split(float x, float y, uint32_t& hi, uint32_
     const float2 h = ka_pair(hi);
     lo = ka_pack(x - h.x, y - h.y);
 }
-__device__ __forceinline__ void ka_scale(uint32_t hi, uint32_t lo, uint32_t scale, uint32_t up, uint32_t& first, uint32_t& rest) {
-    const __half2 h = *reinterpret_cast<const __half2*>(&hi), l = *reinterpret_cast<const __half2*>(&lo);
-    const __half2 s = __hmul2(*reinterpret_cast<const __half2*>(&scale), *reinterpret_cast<const __half2*>(&up)), f = __hmul2(h, s), r = __hfma2(l, s, __hfma2(h, s, __hneg2(f)));
-    first = *reinterpret_cast<const uint32_t*>(&f);
-    rest = *reinterpret_cast<const uint32_t*>(&r);
-}
-// exponent of a scale from its fp16 bits: below 2^(e + 1); scales below 2^-14 count as that
-__device__ __forceinline__ int ka_exponent(uint32_t bits) { return max((int)(bits >> 10), 1) - 15; }
 
 struct ka_item { int r, kv, z, tile, tiles; }; // a place in the line of tiles
 
@@ -81,7 +74,9 @@ struct ka_item { int r, kv, z, tile, tiles; }; // a place in the line of tiles
 #define KA_ITEM ((uint32_t)LB_KV4_ITEM)
 #define KA_LIFT 4.f  // probabilities are 2^4 at their reference
 #define KA_OVER 6.f  // and may pass it by 2^6
-#define KA_WIDE 0x14001400u // a scale may pass its group's reference by 2^5: fp16 bits
+#define KA_WEIGHT 9  // a column's largest weight, probability times scale, is brought to [2^9, 2^10)
+#define KA_ROOM 6    // and later ones may be as large as 2^15
+#define KA_LEAST -110 // weights count as no smaller than 2^-110 for that
 
 template <int D>
 struct ka {
@@ -91,7 +86,7 @@ struct ka {
     struct alignas(128) smem {
         unsigned char ring[NS][BLOCKS * BLK];
         union {
-            uint4 p[P_BUFS][BLOCKS][32];        // probabilities in two terms, a block's as a lane has them
+            float4 p[P_BUFS][BLOCKS][32];       // probabilities, a block's as a lane has them
             float sum[PARTS][KA_COLS][D + 4];   // at an item's end
         };
         uint4 q[4 * S][32];             // queries likewise: step 4 group + 2 word + u
@@ -276,9 +271,8 @@ struct ka {
     float m;            // reference of column g's scores, in log2 units
     float low[4];       // of this warp's rows, column g in two terms: sums of p lowest of groups 2 ft, 2 ft + 1; ft = 2: the sum of p
     float acc[8][2];    // of this warp's group and part, column g: features 8 (2 ft, 2 ft + 1) + j: of a for even j, of a + 16 b for odd ones
-    uint32_t ref;       // fp16 bits, twice, of the scale that this warp's are taken against
-    uint32_t room;      // and of the largest that they may be
-    uint32_t up;        // fp16 2^-1 over the reference's power of two, twice
+    float room;         // of column g's weights in this warp: how large they may be, a power of two, or 0 before the first
+    float up;           // what brings them to fp16's range: 2^15 / room, or 0
     float f;            // of column g's scores
     int len, first_new; // rows of the item, the first of its new ones
 
@@ -289,7 +283,7 @@ struct ka {
         low[0] = low[1] = low[2] = low[3] = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = 0.f;
-        ref = room = up = 0u;
+        room = up = 0.f;
     }
 
     // (scale, lowest) of four rows, of those that are there
@@ -304,27 +298,24 @@ struct ka {
     };
 
     // scores -> probabilities, for whoever reads the block out
-    __device__ __forceinline__ void weigh(rows& r, uint4* to) {
+    __device__ __forceinline__ void weigh(rows& r, float4* to) {
         const float less = KA_LIFT - (m == -INFINITY ? 0.f : m); // a column that has seen nothing yet
         float pr[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) pr[i] = ka_exp2(fmaf(r.sc[i], f, less));
         ka_split(pr[0], pr[1], r.hi.x, r.lo.x);
         ka_split(pr[2], pr[3], r.hi.y, r.lo.y);
-        to[lane] = make_uint4(r.hi.x, r.lo.x, r.hi.y, r.lo.y);
+        to[lane] = make_float4(pr[0], pr[1], pr[2], pr[3]);
     }
-    // a new reference for the scales of this warp's group
-    __device__ __forceinline__ void widen(uint32_t v) {
-        v = __vmaxu2(v, __shfl_xor_sync(0xffffffffu, v, 1));
-        v = __vmaxu2(v, __shfl_xor_sync(0xffffffffu, v, 2));
-        v = max(v & 0xffffu, v >> 16);
-        const int before = ka_exponent(ref & 0xffffu);
-        ref = max(ref & 0xffffu, v) * 0x10001u;
-        room = ref ? __vaddus2(ref, KA_WIDE) : 0u;
-        const int e = ka_exponent(ref & 0xffffu);
-        const float shrink = ka_pow2(before - e);
-        const __half2 u = __float2half2_rn(ka_pow2(-1 - e));
-        up = *reinterpret_cast<const uint32_t*>(&u);
+    // `top`: the largest of this thread's weights of a tile.  A new reference for the columns where it is beyond what there is room for
+    __device__ __forceinline__ void widen(float top) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (!(top > room)) return;
+        const int e = max((__float_as_int(top) >> 23) - 127, KA_LEAST);
+        const float shrink = room * ka_pow2(-(e + KA_ROOM)); // 0 before the first, when there are no sums yet
+        room = ka_pow2(e + KA_ROOM);
+        up = ka_pow2(KA_WEIGHT - e);
 #pragma unroll
         for (int j = 0; j < 8; ++j) { acc[j][0] *= shrink; acc[j][1] *= shrink; }
     }
@@ -333,7 +324,7 @@ struct ka {
     template <bool FULL>
     __device__ __forceinline__ bool tile(const ka_item& it, uint32_t i_tile, uint32_t tiles) {
         const int slot = i_tile % NS, nb = FULL ? BLOCKS : min(BLOCKS, (len - it.tile * TILE + 15) >> 4), row0 = it.tile * TILE + 4 * ft, group = warp % S, part = warp / S;
-        uint4 (*const pw)[32] = s.p[P_BUFS == 2 ? i_tile & 1 : 0];
+        float4 (*const pw)[32] = s.p[P_BUFS == 2 ? i_tile & 1 : 0];
         const unsigned char* ring = s.ring[slot];
         rows r[BW];
         bool landed = mbar_wait(&s.full[slot], (i_tile / NS) & 1), over = !landed;
@@ -405,7 +396,7 @@ struct ka {
 #pragma unroll
             for (int k = 0; k < BW; ++k) weigh(r[k], pw[warp + 8 * k]);
         // the values' scales of the blocks that this warp reads out
-        uint32_t s01[4], s23[4], wide = 0u;
+        uint32_t s01[4], s23[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int b = k * PARTS + part;
@@ -415,18 +406,12 @@ struct ka {
             if (!FULL) v = there(v, row0 + 16 * b, len);
             s01[k] = __byte_perm(v.x, v.y, 0x5410);
             s23[k] = __byte_perm(v.z, v.w, 0x5410);
-            if (FULL) wide = __vmaxu2(wide, __vmaxu2(s01[k], s23[k]));
-            else { // a NaN has no say here: columns before its row are not to notice it
-                wide = __vmaxu2(wide, s01[k] & __vcmpltu2(s01[k], 0x7c007c00u));
-                wide = __vmaxu2(wide, s23[k] & __vcmpltu2(s23[k], 0x7c007c00u));
-            }
             if (!FULL) { // a NaN's group reaches the columns that see its row, and no other as 0 times NaN
                 const int lim = s.limit[g] - row0 - 16 * b;
                 s01[k] &= (lim >= 0 ? 0xffffu : 0u) | (lim >= 1 ? 0xffff0000u : 0u);
                 s23[k] &= (lim >= 2 ? 0xffffu : 0u) | (lim >= 3 ? 0xffff0000u : 0u);
             }
         }
-        if (__any_sync(0xffffffffu, wide != __vminu2(wide, room))) widen(wide); // a reference of 0 has no room
         if (__syncthreads_or(over || !landed)) {
             if (__syncthreads_or(!landed)) return false;
             renew(r, FULL || warp < nb, pw);
@@ -442,7 +427,28 @@ struct ka {
             lv[k][0] = g == 4 ? 0x3c003c00u : __byte_perm(vr.x, vr.y, 0x7632);
             lv[k][1] = g == 4 ? 0x3c003c00u : __byte_perm(vr.z, vr.w, 0x7632);
         }
+        auto lowest = [&] {
+#pragma unroll
+            for (int k = 0; k < BW; ++k) {
+                float d[4];
+                ka_mma0(d, make_uint4(r[k].hi.x, r[k].lo.x, r[k].hi.y, r[k].lo.y), lv[k][0], lv[k][1]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) low[i] += d[i];
+            }
+        };
+        if (BW > 2) lowest(); // frees their registers
         if (FULL || part < nb) {
+            // weights, in 32 bits: a scale says nothing about them where the probability is small.  A NaN has no say in their reference
+            float w[4][4], top = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int b = k * PARTS + part;
+                const float4 pk = !FULL && b >= nb ? make_float4(0.f, 0.f, 0.f, 0.f) : pw[b][lane];
+                const float2 x = ka_pair(s01[k]), y = ka_pair(s23[k]);
+                w[k][0] = pk.x * x.x; w[k][1] = pk.y * x.y; w[k][2] = pk.z * y.x; w[k][3] = pk.w * y.y;
+                top = fmaxf(fmaxf(top, fmaxf(w[k][0], w[k][1])), fmaxf(w[k][2], w[k][3]));
+            }
+            if (__any_sync(0xffffffffu, top > room)) widen(top);
             float d[8][4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -450,11 +456,9 @@ struct ka {
                 if (!FULL && k && b >= nb) break;
                 const uint4 v = *reinterpret_cast<const uint4*>(ring + b * BLK + 8 * D + group * 512 + lane * 16);
                 const uint32_t a0 = __byte_perm(v.x, v.y, 0x5410), a1 = __byte_perm(v.x, v.y, 0x7632), c0 = __byte_perm(v.z, v.w, 0x5410), c1 = __byte_perm(v.z, v.w, 0x7632);
-                // (hi + lo) scale in two terms: the first product rounded, what the rounding left exactly, and lo scale on top of that
-                const uint4 pk = pw[b][lane];
                 uint4 pa;
-                ka_scale(pk.x, pk.y, s01[k], up, pa.x, pa.y);
-                ka_scale(pk.z, pk.w, s23[k], up, pa.z, pa.w);
+                ka_split(w[k][0] * up, w[k][1] * up, pa.x, pa.y);
+                ka_split(w[k][2] * up, w[k][3] * up, pa.z, pa.w);
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const uint32_t y = j < 4 ? a0 : a1, z = j < 4 ? c0 : c1;
@@ -475,13 +479,7 @@ struct ka {
                 acc[j][1] += d[j][1] + d[j][3];
             }
         }
-#pragma unroll
-        for (int k = 0; k < BW; ++k) {
-            float d[4];
-            ka_mma0(d, make_uint4(r[k].hi.x, r[k].lo.x, r[k].hi.y, r[k].lo.y), lv[k][0], lv[k][1]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) low[i] += d[i];
-        }
+        if (BW <= 2) lowest();
         __syncwarp();
         if (lane == 0) { // whoever finds that all warps are done, the last one at least, requests what comes to this place next
             mbar_arrive(&s.pfree);
@@ -496,7 +494,7 @@ struct ka {
     }
 
     // new references: the exchange of maxima, and the probabilities again
-    __device__ __forceinline__ void renew(rows (&r)[BW], bool live, uint4 (*pw)[32]) {
+    __device__ __forceinline__ void renew(rows (&r)[BW], bool live, float4 (*pw)[32]) {
         float best = -INFINITY;
 #pragma unroll
         for (int k = 0; k < BW; ++k) best = fmaxf(best, fmaxf(fmaxf(r[k].sc[0], r[k].sc[1]), fmaxf(r[k].sc[2], r[k].sc[3])));
@@ -552,8 +550,7 @@ struct ka {
         if (2 * ft + 1 < S) s.part[warp][g][2 * ft + 1] = low[1] + low[3];
         if (ft == 2) s.part[warp][g][S] = low[0] + low[2];
         if (ft == 0 && warp == 0) s.m[g] = m;
-        const int e = ka_exponent(ref & 0xffffu);
-        const float even = ka_pow2(e + 25), odd = even * 0.0625f; // 2^24 over 2^(-1 - e)
+        const float even = room * ka_pow2(24 - KA_WEIGHT - KA_ROOM), odd = even * 0.0625f; // 2^24 / up
         __syncthreads(); // the probabilities have been read
 #pragma unroll
         for (int i = 0; i < 2; ++i)

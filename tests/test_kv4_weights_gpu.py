@@ -1,0 +1,65 @@
+"""Weights of the batch attention far below the largest, and scales far apart: against 64 bits, with bounds for the 22 bits that the header gives."""
+import numpy as np
+import pytest
+
+import kv4_cases as kc
+from kv4_close import close, rounded
+
+pytestmark = pytest.mark.gpu
+
+
+def rows_case(ctx, dim, length, new, below, scale, seed, heads=2):
+    """One sequence whose row t has a score below[t] under 0 in log2 units (and 0.1 to both sides) and values of scale scale[t]"""
+    case = kc.Case(ctx, dim, heads, 2, -(-length // 16) * 16, seqs=[1], pos=[length - new], new=[new], seed=seed)
+    S, rows = dim // 64, case.max_ctx
+    rng = np.random.default_rng(seed)
+    fill = lambda a: np.concatenate([a, np.zeros(rows - len(a))]).reshape(1, rows // 16, 1, 16)  # noqa: E731
+    pairs = case.cache[1, :, :, 16 * dim:].copy().view(np.float16).reshape(heads, rows // 16, 2, S, 16, 2)
+    shape = pairs.shape[:2] + pairs.shape[3:5]
+    pairs[:, :, 0, :, :, 0] = 0.02 / 15 * rng.random(shape)
+    pairs[:, :, 0, :, :, 1] = np.broadcast_to(fill(-np.asarray(below) * np.log(2) / np.sqrt(dim)), shape)
+    s = fill(np.asarray(scale, np.float64)) * (0.5 + rng.random(shape))
+    pairs[:, :, 1, :, :, 0] = s.clip(max=8700)
+    pairs[:, :, 1, :, :, 1] = (s * (rng.random(shape) - 7.5)).clip(-65504, 65504)
+    case.cache[1, :, :, 16 * dim:] = pairs.view(np.uint8).reshape(heads, rows // 16, -1)
+    case.d_cache.upload(case.cache)
+    return case
+
+
+def check(lb, ctx, case, G, seed=3, tokens=None):
+    rng, D, HQ, new = np.random.default_rng(seed), case.dim, case.heads * G, case.new[0]
+    q = 0.5 + rng.random((new, HQ, D))
+    q = (q * D / q.sum(-1, keepdims=True)).astype(np.float32)
+    d_q, out = ctx.to_device(q), ctx.alloc(new * HQ * D * 2)
+    ctx.kv4_attention(case.desc, case.batch, d_q, None, 0, 0, lb.IN_F32, None, out, HQ, new, 0, 1e7, 1e-6)
+    got = out.download(np.float16).astype(np.float64).reshape(new, HQ, D)
+    assert ctx.device_status() == 0
+    for h in range(HQ):
+        rows = kc.cache_rows(case.cache, D, 1, h // G, case.pos[0] + new)
+        for i in range(new) if tokens is None else tokens:
+            want, tol = close(q[i, h].astype(np.float64), *rows, case.pos[0] + i)
+            err, tol = np.abs(got[i, h] - want), rounded(want, tol)
+            assert (err <= tol).all(), (i, h, float((err / tol).max()), float(np.linalg.norm(got[i, h] - want) / np.linalg.norm(want)))
+    for b in (d_q, out):
+        b.free()
+    case.free()
+
+
+@pytest.mark.parametrize("where", ["first", "middle", "last"])
+@pytest.mark.parametrize("large,small", [(300, 0.05), (3000, 0.02), (8700, 0.01)])
+@pytest.mark.parametrize("dim,length,new", [(64, 500, 1), (64, 1800, 5), (128, 900, 5), (256, 100, 1), (256, 700, 1)])
+def test_row_of_large_values_without_weight(lb, ctx, dim, length, new, large, small, where):
+    """a row 60 below the largest score has values of another order of magnitude: the others keep their bits"""
+    below, scale = np.random.default_rng(1).uniform(0, 6, length), np.full(length, float(small))
+    row = {"first": 0, "middle": length // 2, "last": length - new}[where]
+    below[row], scale[row] = 60, large
+    check(lb, ctx, rows_case(ctx, dim, length, new, below, scale, seed=dim + length), 3)
+
+
+@pytest.mark.parametrize("dim,length,new", [(64, 1500, 1), (128, 700, 3), (256, 600, 1)])
+def test_large_values_behind_a_row_that_has_none(lb, ctx, dim, length, new):
+    """the top score's values are 0, those of a row without weight are large: what is left are rows 20 below the one, of a millionth of the other's size"""
+    below, scale = np.random.default_rng(2).uniform(20, 22, length), np.full(length, 0.01)
+    below[0], scale[0] = 0, 0
+    below[5], scale[5] = 70, 8700
+    check(lb, ctx, rows_case(ctx, dim, length, new, below, scale, seed=dim), 4)
