@@ -6,8 +6,9 @@
 //     rate.  A byte holds two codes a, b; a alone (a & 15) and both (a + 16 b) go in, two instructions a byte pair and no conversion, and b is had by difference:
 //     q0 a + q1 b = (q0 - q1 / 16) a + (q1 / 16) (a + 16 b), and of the read-outs after the sums.  scores = sum over groups of scale_t (q . c_t) + lowest_t sum(q);
 //     read-out = sum of (p_t scale_t) c_t + p_t lowest_t.
-//   * q and p scale go in as two fp16 terms, the leading one in rows 0..7 of a product and what it leaves in rows 8..15: 22 bits of each, for the price of rows that eight
-//     columns would leave empty.  A query is scaled by a power of two to [2^13, 2^14) at its largest.  Scores, sums and read-outs are fp32, a tile's read-outs added up
+//   * q, p and p scale go in as two fp16 terms, the leading one in rows 0..7 of a product and what it leaves in rows 8..15: 22 bits of each, for the price of rows that eight
+//     columns would leave empty.  Weights are 2^9 at their reference and their second terms go in 2^11 up, so that the 22 bits reach down to 2^-23 of it; below that 2^-45 of
+//     it stays, which many rows far below one that has the top score and small values need.  A query is scaled by a power of two to [2^13, 2^14) at its largest.  Scores, sums and read-outs are fp32, a tile's read-outs added up
 //     by themselves (the products' own additions cut off); the output is fp16, what lb_gemm_int4 takes.
 //   * lowest_t sum(q) is one product more per 8 rows, p_t lowest_t and the sum of p one per 16.
 //   * A tile is 32768 / D rows, 36 KB, one bulk copy, requested by whichever warp is the last to be done with the place it goes to.  A warp does the scores of 256 / D blocks of
@@ -68,11 +69,29 @@ __device__ __forceinline__ void ka_split(float x, float y, uint32_t& hi, uint32_
     lo = ka_pack(x - h.x, y - h.y);
 }
 
+// the same with the second term carried 2^11 up, where a small number's still has its bits: its products have sums of their own
+#define KA_REST 4.8828125e-04f // 2^-11
+__device__ __forceinline__ float2 ka_mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 ka_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ void ka_split_up(float2 v, uint32_t& hi, uint32_t& lo) {
+    hi = ka_pack(v.x, v.y);
+    const float2 up = make_float2(1.f / KA_REST, 1.f / KA_REST), r = ka_fma2(ka_pair(hi), make_float2(-1.f / KA_REST, -1.f / KA_REST), ka_mul2(v, up));
+    lo = ka_pack(r.x, r.y);
+}
+
 struct ka_item { int r, kv, z, tile, tiles; }; // a place in the line of tiles
 
 #define KA_STEP ((uint32_t)LB_KV4_STEP)
 #define KA_ITEM ((uint32_t)LB_KV4_ITEM)
-#define KA_LIFT 4.f  // probabilities are 2^4 at their reference
+#define KA_LIFT 9.f  // probabilities are 2^9 at their reference
 #define KA_OVER 6.f  // and may pass it by 2^6
 #define KA_WEIGHT 9  // a column's largest weight, probability times scale, is brought to [2^9, 2^10)
 #define KA_ROOM 6    // and later ones may be as large as 2^15
@@ -269,7 +288,7 @@ struct ka {
     }
 
     float m;            // reference of column g's scores, in log2 units
-    float low[4];       // of this warp's rows, column g in two terms: sums of p lowest of groups 2 ft, 2 ft + 1; ft = 2: the sum of p
+    float low[4];       // of this warp's rows, column g, from first and from second terms: sums of p lowest of groups 2 ft, 2 ft + 1; ft = 2: the sum of p
     float acc[8][2];    // of this warp's group and part, column g: features 8 (2 ft, 2 ft + 1) + j: of a for even j, of a + 16 b for odd ones
     float room;         // of column g's weights in this warp: how large they may be, a power of two, or 0 before the first
     float up;           // what brings them to fp16's range: 2^15 / room, or 0
@@ -303,8 +322,8 @@ struct ka {
         float pr[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) pr[i] = ka_exp2(fmaf(r.sc[i], f, less));
-        ka_split(pr[0], pr[1], r.hi.x, r.lo.x);
-        ka_split(pr[2], pr[3], r.hi.y, r.lo.y);
+        ka_split_up(make_float2(pr[0], pr[1]), r.hi.x, r.lo.x);
+        ka_split_up(make_float2(pr[2], pr[3]), r.hi.y, r.lo.y);
         to[lane] = make_float4(pr[0], pr[1], pr[2], pr[3]);
     }
     // `top`: the largest of this thread's weights of a tile.  A new reference for the columns where it is beyond what there is room for
@@ -439,14 +458,15 @@ struct ka {
         if (BW > 2) lowest(); // frees their registers
         if (FULL || part < nb) {
             // weights, in 32 bits: a scale says nothing about them where the probability is small.  A NaN has no say in their reference
-            float w[4][4], top = 0.f;
+            float2 w[4][2];
+            float top = 0.f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int b = k * PARTS + part;
                 const float4 pk = !FULL && b >= nb ? make_float4(0.f, 0.f, 0.f, 0.f) : pw[b][lane];
-                const float2 x = ka_pair(s01[k]), y = ka_pair(s23[k]);
-                w[k][0] = pk.x * x.x; w[k][1] = pk.y * x.y; w[k][2] = pk.z * y.x; w[k][3] = pk.w * y.y;
-                top = fmaxf(fmaxf(top, fmaxf(w[k][0], w[k][1])), fmaxf(w[k][2], w[k][3]));
+                w[k][0] = ka_mul2(make_float2(pk.x, pk.y), ka_pair(s01[k]));
+                w[k][1] = ka_mul2(make_float2(pk.z, pk.w), ka_pair(s23[k]));
+                top = fmaxf(fmaxf(top, fmaxf(w[k][0].x, w[k][0].y)), fmaxf(w[k][1].x, w[k][1].y));
             }
             if (__any_sync(0xffffffffu, top > room)) widen(top);
             float d[8][4];
@@ -457,8 +477,8 @@ struct ka {
                 const uint4 v = *reinterpret_cast<const uint4*>(ring + b * BLK + 8 * D + group * 512 + lane * 16);
                 const uint32_t a0 = __byte_perm(v.x, v.y, 0x5410), a1 = __byte_perm(v.x, v.y, 0x7632), c0 = __byte_perm(v.z, v.w, 0x5410), c1 = __byte_perm(v.z, v.w, 0x7632);
                 uint4 pa;
-                ka_split(w[k][0] * up, w[k][1] * up, pa.x, pa.y);
-                ka_split(w[k][2] * up, w[k][3] * up, pa.z, pa.w);
+                ka_split_up(ka_mul2(w[k][0], make_float2(up, up)), pa.x, pa.y);
+                ka_split_up(ka_mul2(w[k][1], make_float2(up, up)), pa.z, pa.w);
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const uint32_t y = j < 4 ? a0 : a1, z = j < 4 ? c0 : c1;
@@ -475,8 +495,8 @@ struct ka {
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                acc[j][0] += d[j][0] + d[j][2];
-                acc[j][1] += d[j][1] + d[j][3];
+                acc[j][0] += fmaf(d[j][2], KA_REST, d[j][0]);
+                acc[j][1] += fmaf(d[j][3], KA_REST, d[j][1]);
             }
         }
         if (BW <= 2) lowest();
@@ -505,11 +525,16 @@ struct ka {
         const float4 a = *reinterpret_cast<const float4*>(s.max[g]), b = *reinterpret_cast<const float4*>(s.max[g] + 4);
         const float now = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))) * f, top = fmaxf(m, now);
         const float corr = top == -INFINITY ? 0.f : ka_exp2(m - top);
+        // weights to come are smaller by as much: where there are some, their reference follows, and the sums so far stay as large as they are
+        const int down = room > 0.f ? min(min((int)(top - m), (__float_as_int(room) >> 23) - 127 - (KA_LEAST + KA_ROOM)), 100) : 0;
+        const float keep = corr * ka_pow2(down);
+        room *= ka_pow2(-down);
+        up *= ka_pow2(down);
         m = top;
 #pragma unroll
         for (int i = 0; i < 4; ++i) low[i] *= corr;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { acc[j][0] *= corr; acc[j][1] *= corr; }
+        for (int j = 0; j < 8; ++j) { acc[j][0] *= keep; acc[j][1] *= keep; }
         if (live)
 #pragma unroll
             for (int k = 0; k < BW; ++k) weigh(r[k], pw[warp + 8 * k]);
@@ -546,9 +571,9 @@ struct ka {
     // The item's columns, whole or this CTA's share of them.  `first`: the item's first tile was this CTA's, `last`: its last
     __device__ __forceinline__ void finish(const ka_item& it, bool first, bool last) {
         const int group = warp % S, part = warp / S, cols = min(KA_COLS, s.n[it.r] * G - it.z * KA_COLS);
-        if (2 * ft < S) s.part[warp][g][2 * ft] = low[0] + low[2];
-        if (2 * ft + 1 < S) s.part[warp][g][2 * ft + 1] = low[1] + low[3];
-        if (ft == 2) s.part[warp][g][S] = low[0] + low[2];
+        if (2 * ft < S) s.part[warp][g][2 * ft] = fmaf(low[2], KA_REST, low[0]);
+        if (2 * ft + 1 < S) s.part[warp][g][2 * ft + 1] = fmaf(low[3], KA_REST, low[1]);
+        if (ft == 2) s.part[warp][g][S] = fmaf(low[2], KA_REST, low[0]);
         if (ft == 0 && warp == 0) s.m[g] = m;
         const float even = room * ka_pow2(24 - KA_WEIGHT - KA_ROOM), odd = even * 0.0625f; // 2^24 / up
         __syncthreads(); // the probabilities have been read

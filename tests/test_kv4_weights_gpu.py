@@ -63,3 +63,22 @@ def test_large_values_behind_a_row_that_has_none(lb, ctx, dim, length, new):
     below[0], scale[0] = 0, 0
     below[5], scale[5] = 70, 8700
     check(lb, ctx, rows_case(ctx, dim, length, new, below, scale, seed=dim), 4)
+
+
+@pytest.mark.parametrize("where", ["first", "later"])
+@pytest.mark.parametrize("gap,spread", [(12, 0), (16.3, 0), (18.3, 0), (18.3, 4), (24, 0), (28, 8)])
+@pytest.mark.parametrize("dim,length,new", [(64, 4096, 1), (128, 4096, 2), (256, 4096, 1), (256, 700, 5)])
+def test_rows_far_below_the_largest(lb, ctx, dim, length, new, gap, spread, where):
+    """one row has the top score and values of 0; the result is the others', all `gap` below it or up to `spread` more"""
+    below, scale = gap + spread * np.random.default_rng(3).random(length), np.full(length, 100.0)
+    row = 0 if where == "first" else length - 100
+    below[row], scale[row] = 0, 0
+    check(lb, ctx, rows_case(ctx, dim, length, new, below, scale, seed=dim + new), 3)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_rows_far_below_the_largest(lb, ctx, dim):
+    for gap in (16.3, 20.0):
+        below, scale = np.full(100001, gap), np.full(100001, 100.0)
+        below[0], scale[0] = 0, 0
+        check(lb, ctx, rows_case(ctx, dim, 100001, 1, below, scale, seed=dim, heads=1), 1)
