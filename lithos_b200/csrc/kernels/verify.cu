@@ -62,10 +62,12 @@ struct vd_exps {
         for (int i = threadIdx.x; i < VD_STEPS; i += blockDim.x) table[i] = exp2((double)i / VD_STEPS);
     }
     __device__ __forceinline__ vd_exps(const double* t, float max, double temperature) : table(t) {
-        const bool infinite = max == INFINITY; // those that share it have exp = 1
-        scale = infinite ? 0.0 : VD_STEPS * VD_LOG2E / temperature;
-        less = infinite ? 0.0 : (double)max * scale;
-        low = infinite ? max : max > -INFINITY ? (float)fmax((double)max - 693.0 * temperature, -3.4028234e38) : NAN;
+        // an infinite maximum, or one so far from 0 that the type's next number is 2^15 T off: those that share it have exp = 1, the others 0
+        // (up to there the rounding of `less`, a factor that all exponentials share, is within a step)
+        const bool alone = max == INFINITY || fabs((double)max) > 1099511627776.0 * temperature;
+        scale = alone ? 0.0 : VD_STEPS * VD_LOG2E / temperature;
+        less = alone ? 0.0 : (double)max * scale;
+        low = !(max > -INFINITY) ? NAN : alone ? max : __double2float_ru((double)max - 693.0 * temperature);
     }
     // N at a time, step by step: every operation waits for the one before, so others have to be under way
     template <int N>
