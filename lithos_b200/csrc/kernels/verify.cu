@@ -57,7 +57,7 @@ __device__ __forceinline__ double vd_double(float v) {
 struct vd_exps {
     double scale, less; // y = l * scale - less
     const double* table;
-    float low;          // what lies below adds nothing (2^-1000); a NaN where there is no logit at all
+    float low;          // what lies below, 2^-969, adds nothing (above it a probability, 2^-24 and less of that, has an exponent); a NaN where there is no logit at all
     __device__ __forceinline__ static void fill(double* table) { // a barrier follows
         for (int i = threadIdx.x; i < VD_STEPS; i += blockDim.x) table[i] = exp2((double)i / VD_STEPS);
     }
@@ -67,7 +67,7 @@ struct vd_exps {
         const bool alone = max == INFINITY || fabs((double)max) > 1099511627776.0 * temperature;
         scale = alone ? 0.0 : VD_STEPS * VD_LOG2E / temperature;
         less = alone ? 0.0 : (double)max * scale;
-        low = !(max > -INFINITY) ? NAN : alone ? max : __double2float_ru((double)max - 693.0 * temperature);
+        low = !(max > -INFINITY) ? NAN : alone ? max : __double2float_ru((double)max - 672.0 * temperature);
     }
     // N at a time, step by step: every operation waits for the one before, so others have to be under way
     template <int N>
