@@ -3,7 +3,8 @@
 //   Draft x of a row stands while  u q(x) < p(x).  The first row of a request that does not stand, or its last row, which has no draft, gives the token: the
 //   first one whose cumulative weight exceeds u' times their sum, the weights being max(p - q, 0) (at the last row p).
 // What a token's choice depends on is computed in 64 bits: a border between two of 250 000 tokens lies within 2^-24 of some number often enough that 32 bits would pick a neighbour
-// in one draw of a hundred.  Whether a draft stands has a single border; there the sum of a row is one of 32-bit exponentials in 64 bits (2^-24 of it).
+// in one draw of a hundred.  Whether a draft stands has a single border; there the sum of a row is one of 32-bit exponentials, four to a 64-bit addition.  Where logits x
+// under the maximum in log2 units carry it, it is off by 2^-22 for the exponential, 2^-24.5 x for its argument's factor and up to 2^-20.5 (x < 32) for the argument: 2^-19 of itself at most.
 // Two launches: every row by a cluster of up to 8 CTAs, then every request.  The first reads the logits once and is bound by that where there are many rows (5 TB/s at 188 rows of
 // 248 320); the second reads one row of each request again, and of q the row of a draft that fell, and is bound by the issue slots of its exponentials, 45 a logit and warp.
 // us a call at a vocabulary of 248 320: 1 request with 4 drafts 19; 48 with up to 5 and the draft's probabilities 86 (37 and 49); 16 with up to 4, top 50, 28; greedy, 32 with up to
@@ -151,8 +152,8 @@ __device__ __forceinline__ void vd_rows_body(const lb_vd_params& p) {
     const float* x = p.logits + (size_t)row * p.V;
     const int per = (((p.V + C - 1) / C) + 3) & ~3, a = min(p.V, rank * per), b = min(p.V, a + per);
     const float k = GREEDY ? 0.f : (float)(VD_LOG2E / p.temperature);
-    float m = -INFINITY, sum = 0.f;
-    double ref = 0.0; // the sum's reference
+    float m = -INFINITY;
+    double sum = 0.0, ref = 0.0; // the sum and its reference
     int best = 0x7fffffff;
     if (GREEDY) {
         vd_each<VD_THREADS>(x, a, b, [&](const float4& v, int i) {
@@ -163,30 +164,27 @@ __device__ __forceinline__ void vd_rows_body(const lb_vd_params& p) {
             }
         });
     } else {
-        float s[2] = {0.f, 0.f}, c = 0.f;
+        float c = 0.f;
         vd_each<VD_THREADS>(x, a, b, [&](const float4& v, int) {
             const float mx = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
             if (mx > m) {
                 const float now = fmaxf(-3.4e38f, mx * k), d = c - now;
-                if (m == -INFINITY || d < -24.f) { // 2^24 times 2^24 logits fit fp32
-                    s[0] *= m == -INFINITY ? 0.f : vd_exp2(d);
-                    s[1] *= m == -INFINITY ? 0.f : vd_exp2(d);
+                if (m == -INFINITY || d < -24.f) { // four of 2^24 fit fp32
+                    sum *= m == -INFINITY ? 0.0 : (double)vd_exp2(d);
                     c = now;
                 }
                 m = mx;
             }
-            s[0] += vd_exp2(fmaf(v.x, k, -c)) + vd_exp2(fmaf(v.y, k, -c));
-            s[1] += vd_exp2(fmaf(v.z, k, -c)) + vd_exp2(fmaf(v.w, k, -c));
+            sum += (double)((vd_exp2(fmaf(v.x, k, -c)) + vd_exp2(fmaf(v.y, k, -c))) + (vd_exp2(fmaf(v.z, k, -c)) + vd_exp2(fmaf(v.w, k, -c))));
         });
-        sum = s[0] + s[1];
         ref = (double)c;
         if (!(sum < INFINITY) || !(fabsf(m * k) < 16777216.f)) { // NaN logits; infinite ones, of which only those that share the maximum count; a c that is known to whole numbers only
-            sum = 0.f;
+            sum = 0.0;
             ref = (double)m * (double)k;
             auto one = [&](float l) { return l == m ? 1.f : l < m ? vd_exp2((l - m) * k) : 0.f; };
-            vd_each<VD_THREADS>(x, a, b, [&](const float4& v, int) { sum += one(v.x) + one(v.y) + one(v.z) + one(v.w); });
+            vd_each<VD_THREADS>(x, a, b, [&](const float4& v, int) { sum += (double)((one(v.x) + one(v.y)) + (one(v.z) + one(v.w))); });
         }
-        if (m == -INFINITY) sum = 0.f;
+        if (m == -INFINITY) sum = 0.0;
     }
     const vd_place at = vd_find(p, row);
     if (!at.covered) return; // the same for the whole cluster
@@ -212,7 +210,7 @@ __device__ __forceinline__ void vd_rows_body(const lb_vd_params& p) {
     }
     double S = 0.0;
     if (!GREEDY) {
-        if (sum > 0.f) S = M == INFINITY ? (m == M ? (double)sum : 0.0) : (double)sum * exp2(ref - (double)M * (double)k);
+        if (sum > 0.0) S = M == INFINITY ? (m == M ? sum : 0.0) : sum * exp2(ref - (double)M * (double)k);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) S += __shfl_xor_sync(0xffffffffu, S, o);
         if (lane == 0) ss[warp] = S;

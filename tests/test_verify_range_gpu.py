@@ -37,3 +37,27 @@ def test_verify_longest_vocabulary(lb, ctx):
             run(lb, ctx, c, 1.0, 0, probs, tol=2.0 ** -14)
     q[0] = 0.5  # nothing is left of p: from p itself
     run(lb, ctx, c, 1.0, 0, tol=2.0 ** -14)
+
+
+@pytest.mark.parametrize("V,rows", [(248320, 192), (50257, 300), (32768, 8), (1 << 24, 5)])
+def test_verify_long_sums(lb, ctx, V, rows):
+    """p to 2^-19 of itself where it hangs on a long sum: most of a row's weight in logits alike, some way below a few"""
+    rng = np.random.default_rng(33)
+    gap = np.linspace(1, 17, rows)
+    l = np.zeros((rows, V), np.float32)
+    for i in range(rows):
+        l[i, rng.integers(0, V, 3)] = gap[i]
+    drafts = rng.integers(0, V, rows).astype(np.int32)
+    u = np.full(rows, 0.5, np.float32)
+    s, d = ctx.to_device(np.array([0, rows], np.int32)), {k: ctx.to_device(a) for k, a in (("l", l), ("d", drafts), ("u", u))}
+    tokens, accepted, p = ctx.alloc(4 * rows), ctx.alloc(4), ctx.alloc(4 * rows)
+    for temperature in (1.0, 0.7, 1.3):
+        ctx.verify_drafts(d["l"], V, s, 1, rows, d["d"], None, d["u"], d["u"], tokens, accepted, temperature, 0, p)
+        got, worst = p.download(np.float32), 0.0
+        for i in range(rows - 1):
+            x = l[i].astype(np.float64) / temperature
+            want = np.exp(x[drafts[i]] - x.max()) / np.exp(x - x.max()).sum()
+            worst = max(worst, abs(got[i] / want - 1))
+        assert worst <= 2.0 ** -19, np.log2(worst)
+    for b in (s, *d.values(), tokens, accepted, p):
+        b.free()
