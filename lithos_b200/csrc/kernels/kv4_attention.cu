@@ -258,7 +258,7 @@ struct ka {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         int e = 13 - ((__float_as_int(top) >> 23) - 127); // largest to [2^13, 2^14)
-        e = top == 0.f ? 0 : min(120, max(-100, e));
+        e = top == 0.f ? 0 : min(120, max(-114, e));
         const float up = ka_pow2(e);
         float sum = 0.f;
         if (lane < D / 8) {
@@ -282,17 +282,17 @@ struct ka {
             s.qsum[c * 4 + lane] = w;
         }
         if (lane == 0) {
-            s.factor[c] = ka_pow2(24 - e) * (rsqrtf((float)D) * 1.4426950408889634f); // scores in log2 units
+            s.factor[c] = ka_pow2(min(24 - e, 127)) * (rsqrtf((float)D) * 1.4426950408889634f); // scores in log2 units; of queries beyond 2^115 less than those: one row has all the weight
             s.limit[c] = on ? pos + i : -1;
         }
     }
 
-    float m;            // reference of column g's scores, in log2 units
+    float m;            // reference of column g's scores: one of them, so that its own difference is 0 whatever its size
     float low[4];       // of this warp's rows, column g, from first and from second terms: sums of p lowest of groups 2 ft, 2 ft + 1; ft = 2: the sum of p
     float acc[8][2];    // of this warp's group and part, column g: features 8 (2 ft, 2 ft + 1) + j: of a for even j, of a + 16 b for odd ones
     float room;         // of column g's weights in this warp: how large they may be, a power of two, or 0 before the first
     float up;           // what brings them to fp16's range: 2^15 / room, or 0
-    float f;            // of column g's scores
+    float f;            // of column g's scores, to log2 units
     int len, first_new; // rows of the item, the first of its new ones
 
     __device__ __forceinline__ void begin(const ka_item& it) {
@@ -318,10 +318,10 @@ struct ka {
 
     // scores -> probabilities, for whoever reads the block out
     __device__ __forceinline__ void weigh(rows& r, float4* to) {
-        const float less = KA_LIFT - (m == -INFINITY ? 0.f : m); // a column that has seen nothing yet
+        const float from = m == -INFINITY ? 0.f : m; // a column that has seen nothing yet
         float pr[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pr[i] = ka_exp2(fmaf(r.sc[i], f, less));
+        for (int i = 0; i < 4; ++i) pr[i] = ka_exp2(fmaf(r.sc[i] - from, f, KA_LIFT));
         ka_split_up(make_float2(pr[0], pr[1]), r.hi.x, r.lo.x);
         ka_split_up(make_float2(pr[2], pr[3]), r.hi.y, r.lo.y);
         to[lane] = make_float4(pr[0], pr[1], pr[2], pr[3]);
@@ -400,7 +400,7 @@ struct ka {
                     for (int i = 0; i < 4; ++i)
                         if (i > lim) r[k].sc[i] = -INFINITY;
                 }
-                over |= fmaf(fmaxf(fmaxf(r[k].sc[0], r[k].sc[1]), fmaxf(r[k].sc[2], r[k].sc[3])), f, -m) > KA_OVER;
+                over |= (fmaxf(fmaxf(r[k].sc[0], r[k].sc[1]), fmaxf(r[k].sc[2], r[k].sc[3])) - m) * f > KA_OVER;
             }
         } else {
 #pragma unroll
@@ -523,10 +523,10 @@ struct ka {
         if (ft == 0) s.max[g][warp] = best;
         __syncthreads();
         const float4 a = *reinterpret_cast<const float4*>(s.max[g]), b = *reinterpret_cast<const float4*>(s.max[g] + 4);
-        const float now = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))) * f, top = fmaxf(m, now);
-        const float corr = top == -INFINITY ? 0.f : ka_exp2(m - top);
+        const float now = fmaxf(fmaxf(fmaxf(a.x, a.y), fmaxf(a.z, a.w)), fmaxf(fmaxf(b.x, b.y), fmaxf(b.z, b.w))), top = fmaxf(m, now);
+        const float corr = top == -INFINITY ? 0.f : ka_exp2((m - top) * f);
         // weights to come are smaller by as much: where there are some, their reference follows, and the sums so far stay as large as they are
-        const int down = room > 0.f ? min(min((int)(top - m), (__float_as_int(room) >> 23) - 127 - (KA_LEAST + KA_ROOM)), 100) : 0;
+        const int down = room > 0.f ? min(min((int)((top - m) * f), (__float_as_int(room) >> 23) - 127 - (KA_LEAST + KA_ROOM)), 100) : 0;
         const float keep = corr * ka_pow2(down);
         room *= ka_pow2(-down);
         up *= ka_pow2(down);
@@ -608,6 +608,7 @@ struct ka {
             if (!(first && last) && f == 0) {
                 rec[c * LB_KV4_REC(D) + D] = s.m[c];
                 rec[c * LB_KV4_REC(D) + D + 1] = l;
+                rec[c * LB_KV4_REC(D) + D + 2] = s.factor[c];
             }
         }
         __syncthreads(); // the sums' place and the queries are free for the next item
@@ -738,7 +739,7 @@ __device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int 
     const bool few = units <= (int)gridDim.x; // a CTA for each
     for (int first = few ? (int)blockIdx.x : (int)blockIdx.x * KM_GROUPS; first < units; first += few ? (int)gridDim.x : (int)gridDim.x * KM_GROUPS) {
         const int unit = few ? first : first + sub, pair = unit / S, f = unit % S * 64 + (t & 15) * 4;
-        float M = -INFINITY, L = 0.f;
+        float M = -INFINITY, L = 0.f, F = 0.f;
         float4 A = make_float4(0.f, 0.f, 0.f, 0.f), gate = A;
         uint16_t* out = nullptr;
         if (unit < units) {
@@ -759,6 +760,7 @@ __device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int 
                     gate = make_float4(kv4_load1(p.gate, at, p.type), kv4_load1(p.gate, at + 1, p.type), kv4_load1(p.gate, at + 2, p.type), kv4_load1(p.gate, at + 3, p.type));
                 }
             }
+            F = __ldcg(p.records + (((size_t)j.first * 2 + 1) * KA_COLS + c) * LB_KV4_REC(D) + D + 2); // the same in all of them
             for (int b = b0; b < b1; b += 8) {
                 float mv[8], lv[8], mx = M;
                 float4 av[8];
@@ -772,11 +774,11 @@ __device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int 
                 }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) mx = fmaxf(mx, mv[k]);
-                const float use = mx == -INFINITY ? 0.f : mx, w = ka_exp2(M - use);
+                const float use = mx == -INFINITY ? 0.f : mx, w = ka_exp2((M - use) * F);
                 L *= w;
                 A.x *= w; A.y *= w; A.z *= w; A.w *= w;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) km_add(A, L, av[k], lv[k], ka_exp2(mv[k] - use));
+                for (int k = 0; k < 8; ++k) km_add(A, L, av[k], lv[k], ka_exp2((mv[k] - use) * F));
                 M = mx;
             }
         }
@@ -791,7 +793,7 @@ __device__ __forceinline__ void kv4_merge_body(const lb_kv4_attn_params& p, int 
                 L = 0.f;
                 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int q = 0; q < KM_GROUPS; ++q) km_add(A, L, red[q * 16 + t], red_l[q], ka_exp2(red_m[q] - use));
+                for (int q = 0; q < KM_GROUPS; ++q) km_add(A, L, red[q * 16 + t], red_l[q], ka_exp2((red_m[q] - use) * F));
             }
             __syncthreads();
         }

@@ -580,7 +580,7 @@ typedef struct {
     double eps;
     double freq[128];
 } lb_kv4_rows_params;
-#define LB_KV4_REC(D) ((D) + 4) /* floats of a column's record: D sums, maximum, sum, pad */
+#define LB_KV4_REC(D) ((D) + 4) /* floats of a column's record: D sums, largest score, sum, the scores' factor to log2 units, pad */
 typedef struct {               /* what a CTA's first item has to do with the CTA before it */
     int32_t first, last;       /* contributors of the item, where the CTA before is the first of them; first < 0: nothing to merge */
     int32_t row0, kv, col0, cols; /* the request's first token row; the item's columns col0.. (token * G + head) */

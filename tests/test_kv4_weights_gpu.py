@@ -82,3 +82,30 @@ def test_many_rows_far_below_the_largest(lb, ctx, dim):
         below, scale = np.full(100001, gap), np.full(100001, 100.0)
         below[0], scale[0] = 0, 0
         check(lb, ctx, rows_case(ctx, dim, 100001, 1, below, scale, seed=dim, heads=1), 1)
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("size", [1e30, 1e35, 2e38])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_queries_as_large_as_their_type(lb, ctx, dim, size, kind):
+    """scores of up to 2^127: one row has all of the weight"""
+    case = kc.Case(ctx, dim, 1, 1, 512, seqs=[0], pos=[400], new=[1])
+    raw, q = kc.typed(size * np.where(np.arange(2 * dim).reshape(2, dim) % dim < 3, [[1.0], [-0.5]], 0.0), kind)
+    d_q, out = ctx.to_device(raw), ctx.alloc(2 * dim * 2)
+    # keys of about a thousandth, so that 3 of them times a query and 1 / sqrt(dim) are a number that 32 bits hold
+    pairs = case.cache[0, 0, :, 16 * dim:].copy().view(np.float16).reshape(-1, 2, dim // 64, 16, 2)
+    pairs[:, 0] *= np.float16(1e-3)
+    case.cache[0, 0, :, 16 * dim:] = pairs.view(np.uint8).reshape(len(pairs), -1)
+    case.d_cache.upload(case.cache)
+    ctx.kv4_attention(case.desc, case.batch, d_q, None, 0, 0, kind, None, out, 2, 1, 0, 1e7, 1e-6)
+    got = out.download(np.float16).astype(np.float64).reshape(2, dim)
+    (kl, ks, kcode), (vl, vs, vc) = kc.cache_rows(case.cache, dim, 0, 0, 401)
+    for h in range(2):
+        s = (kl + ks * kcode) @ (q[h] / size)
+        best = int(s.argmax())
+        assert s[best] - np.delete(s, best).max() > 2.0 ** -20 * np.abs(s).max()  # beyond the scores' own rounding
+        want = (vl + vs * vc)[best]
+        assert (np.abs(got[h] - want) <= rounded(want, 2.0 ** -18 * (np.abs(vl) + 15 * vs)[best])).all()
+    for b in (d_q, out):
+        b.free()
+    case.free()
