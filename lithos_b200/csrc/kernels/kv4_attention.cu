@@ -243,7 +243,16 @@ struct ka {
 #pragma unroll
             for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
             ss = warp_sum(ss);
-            const float r = rsqrtf(ss * (1.0f / D) + p.eps);
+            float r = rsqrtf(ss * (1.0f / D) + p.eps);
+            if (!(ss < INFINITY)) { // squares beyond fp32: of 2^-80 x, beside which eps is nothing
+                ss = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    x[j] *= 8.27180612553028e-25f;
+                    ss = fmaf(x[j], x[j], ss);
+                }
+                r = rsqrtf(warp_sum(ss) * (1.0f / D));
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = x[j] * r * (mine ? bf16_bits_to_f32(p.norm_w[lane * 8 + j]) : 0.f);
         }

@@ -4,6 +4,7 @@ import pytest
 
 import kv4_cases as kc
 from kv4_close import close, rounded
+from test_kv4_gpu import attention
 
 pytestmark = pytest.mark.gpu
 
@@ -108,4 +109,14 @@ def test_queries_as_large_as_their_type(lb, ctx, dim, size, kind):
         assert (np.abs(got[h] - want) <= rounded(want, 2.0 ** -18 * (np.abs(vl) + 15 * vs)[best])).all()
     for b in (d_q, out):
         b.free()
+    case.free()
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("size", [1e15, 1e20, 1e36])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_normalised_queries_of_any_size(lb, ctx, dim, size, kind):
+    """the sum of their squares may be beyond fp32"""
+    case = kc.Case(ctx, dim, 2, 1, 512, seqs=[0], pos=[300], new=[2])
+    attention(lb, ctx, case, 3, kind, norm=True, rot=32, size=size)
     case.free()
