@@ -309,7 +309,8 @@ int lb_kv4_read(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batc
 /* Attention of the batch's new tokens, whose rows are in the cache: token i of request r sees rows 0 .. pos[r] + i.  Several requests
  * may read the same sequence.
  * q and gate (0: none): element type `type`, head h of token row j at j * row_stride + h * head_stride elements (row_stride 0: n_heads * head_stride, head_stride 0: dim); q is
- * normalised per head (q_norm_w; 0: not) and rotated like the keys, and goes in with 22 bits; so do weights, those below 2^-23 of a token's and head's largest with 2^-45 of it.  The result is multiplied by sigmoid(gate).  n_heads: 1 to 16 times
+ * normalised per head (q_norm_w; 0: not) and rotated like the keys, and goes in with 22 bits; so do weights, those below 2^-23 of a token's and head's largest with 2^-45 of it.  Their products with codes are added
+ * 16 features (rows) at a time and cut off at 2^-19 of a code times the largest operand of those.  The result is multiplied by sigmoid(gate).  n_heads: 1 to 16 times
  * kv_heads.  max_new: the most tokens a request of the batch has, 1 .. LB_KV4_MAX_NEW.  out fp16 [rows, n_heads, dim], what lb_gemm_int4 takes; it
  * overlaps none of the inputs.  Refused where n_reqs full sequences of max_new tokens would make 2^32 places of work (some 2^31 tiles of 32768 / dim rows). */
 int lb_kv4_attention(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch* batch, uint64_t q, uint64_t gate, int64_t row_stride, int64_t head_stride, int type,

@@ -2,10 +2,11 @@
 //   out[j, h] = sum_t p_t v_t * sigmoid(gate[j, h]),  p = softmax over the rows t <= position of token j of  q[j, h] . k_t / sqrt(D),
 // q normalised and rotated as the decode attention does it.  The columns of an item (a request's KV head) are its new tokens times the query heads that share the
 // head; eight of them are taken at a time.
-//   * The codes are the products' operands as they are: the four bits in the low end of a half are the subnormal c 2^-24, and the tensor cores take subnormals exactly, at their full
-//     rate.  A byte holds two codes a, b; a alone (a & 15) and both (a + 16 b) go in, two instructions a byte pair and no conversion, and b is had by difference:
-//     q0 a + q1 b = (q0 - q1 / 16) a + (q1 / 16) (a + 16 b), and of the read-outs after the sums.  scores = sum over groups of scale_t (q . c_t) + lowest_t sum(q);
-//     read-out = sum of (p_t scale_t) c_t + p_t lowest_t.
+//   * The codes are the products' operands without a conversion: bits 4..7 of a half are the subnormal c 2^-20, which the tensor cores take at their full rate; a shift (for three of
+//     four codes) and a mask for two.  A product's additions are cut off 2^-25 below the largest operand times 2^-14, the least normal number, whatever the codes are: at 2^-19 of a code.
+//     (Codes in bits 0..3, where a byte's second one is had by difference without a shift, are 4 to 5 % faster and cut off at 2^-15 of a code: results were off by 2^-17 of the
+//     values where one row has most of the weight, and queries kept 15 bits, not 22.  In bits 6..9, another shift and 1.5 %, they would be cut off at 2^-21.)
+//     scores = sum over groups of scale_t (q . c_t) + lowest_t sum(q); read-out = sum of (p_t scale_t) c_t + p_t lowest_t.
 //   * q, p and p scale go in as two fp16 terms, the leading one in rows 0..7 of a product and what it leaves in rows 8..15: 22 bits of each, for the price of rows that eight
 //     columns would leave empty.  Weights are 2^9 at their reference and their second terms go in 2^11 up, so that the 22 bits reach down to 2^-23 of it; below that 2^-45 of
 //     it stays, which many rows far below one that has the top score and small values need.  A query is scaled by a power of two to [2^13, 2^14) at its largest.  Scores, sums and read-outs are fp32, a tile's read-outs added up
@@ -56,6 +57,23 @@ __device__ __forceinline__ float ka_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two at a time
+__device__ __forceinline__ float2 ka_add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 ka_mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 ka_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
 // has the phase completed?  (no waiting)
 __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
     uint32_t ok;
@@ -71,21 +89,14 @@ __device__ __forceinline__ void ka_split(float x, float y, uint32_t& hi, uint32_
 
 // the same with the second term carried 2^11 up, where a small number's still has its bits: its products have sums of their own
 #define KA_REST 4.8828125e-04f // 2^-11
-__device__ __forceinline__ float2 ka_mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 ka_fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
 __device__ __forceinline__ void ka_split_up(float2 v, uint32_t& hi, uint32_t& lo) {
     hi = ka_pack(v.x, v.y);
     const float2 up = make_float2(1.f / KA_REST, 1.f / KA_REST), r = ka_fma2(ka_pair(hi), make_float2(-1.f / KA_REST, -1.f / KA_REST), ka_mul2(v, up));
     lo = ka_pack(r.x, r.y);
 }
+
+// code j of both halves of a word as fp16 numbers 2^-20 c
+__device__ __forceinline__ uint32_t ka_codes(uint32_t v, int j) { return (j == 0 ? v << 4 : j == 1 ? v : j == 2 ? v >> 4 : v >> 8) & 0x00f000f0u; }
 
 struct ka_item { int r, kv, z, tile, tiles; }; // a place in the line of tiles
 
@@ -272,13 +283,12 @@ struct ka {
         float sum = 0.f;
         if (lane < D / 8) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) { // codes n0 n4 and (n0 n1) (n4 n5) of a word's even bytes, n2 n6 and (n2 n3) (n6 n7) of its odd ones
-                const float o0 = x[2 * u + 1] * up * 0.0625f, o1 = x[2 * u + 5] * up * 0.0625f;
+            for (int u = 0; u < 2; ++u) { // codes 2 u and 2 u + 1 of a word's halves
                 uint4 w;
-                ka_split(x[2 * u] * up - o0, x[2 * u + 4] * up - o1, w.x, w.y);
-                ka_split(o0, o1, w.z, w.w);
+                ka_split(x[2 * u] * up, x[2 * u + 4] * up, w.x, w.y);
+                ka_split(x[2 * u + 1] * up, x[2 * u + 5] * up, w.z, w.w);
                 const float2 a = ka_pair(w.x), b = ka_pair(w.y), c2 = ka_pair(w.z), d = ka_pair(w.w);
-                sum += (a.x + a.y) + (b.x + b.y) + 17.f * ((c2.x + c2.y) + (d.x + d.y));
+                sum += ((a.x + a.y) + (b.x + b.y)) + ((c2.x + c2.y) + (d.x + d.y));
                 s.q[(lane >> 3) * 4 + 2 * (lane & 1) + u][c * 4 + ((lane & 7) >> 1)] = w;
             }
         }
@@ -291,14 +301,14 @@ struct ka {
             s.qsum[c * 4 + lane] = w;
         }
         if (lane == 0) {
-            s.factor[c] = ka_pow2(min(24 - e, 127)) * (rsqrtf((float)D) * 1.4426950408889634f); // scores in log2 units; of queries beyond 2^115 less than those: one row has all the weight
+            s.factor[c] = ka_pow2(min(20 - e, 127)) * (rsqrtf((float)D) * 1.4426950408889634f); // scores in log2 units; of queries beyond 2^119 less than those: one row has all the weight
             s.limit[c] = on ? pos + i : -1;
         }
     }
 
     float m;            // reference of column g's scores: one of them, so that its own difference is 0 whatever its size
     float low[4];       // of this warp's rows, column g, from first and from second terms: sums of p lowest of groups 2 ft, 2 ft + 1; ft = 2: the sum of p
-    float acc[8][2];    // of this warp's group and part, column g: features 8 (2 ft, 2 ft + 1) + j: of a for even j, of a + 16 b for odd ones
+    float acc[8][2];    // of this warp's group and part, column g: features 8 (2 ft, 2 ft + 1) + j
     float room;         // of column g's weights in this warp: how large they may be, a power of two, or 0 before the first
     float up;           // what brings them to fp16's range: 2^15 / room, or 0
     float f;            // of column g's scores, to log2 units
@@ -328,12 +338,15 @@ struct ka {
     // scores -> probabilities, for whoever reads the block out
     __device__ __forceinline__ void weigh(rows& r, float4* to) {
         const float from = m == -INFINITY ? 0.f : m; // a column that has seen nothing yet
-        float pr[4];
+        float2 pr[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pr[i] = ka_exp2(fmaf(r.sc[i] - from, f, KA_LIFT));
-        ka_split_up(make_float2(pr[0], pr[1]), r.hi.x, r.lo.x);
-        ka_split_up(make_float2(pr[2], pr[3]), r.hi.y, r.lo.y);
-        to[lane] = make_float4(pr[0], pr[1], pr[2], pr[3]);
+        for (int i = 0; i < 2; ++i) {
+            const float2 x = ka_fma2(ka_add2(make_float2(r.sc[2 * i], r.sc[2 * i + 1]), make_float2(-from, -from)), make_float2(f, f), make_float2(KA_LIFT, KA_LIFT));
+            pr[i] = make_float2(ka_exp2(x.x), ka_exp2(x.y));
+        }
+        ka_split_up(pr[0], r.hi.x, r.lo.x);
+        ka_split_up(pr[1], r.hi.y, r.lo.y);
+        to[lane] = make_float4(pr[0].x, pr[0].y, pr[1].x, pr[1].y);
     }
     // `top`: the largest of this thread's weights of a tile.  A new reference for the columns where it is beyond what there is room for
     __device__ __forceinline__ void widen(float top) {
@@ -379,9 +392,9 @@ struct ka {
                     for (int k = 0; k < BW; ++k)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const uint32_t v = st < 2 ? w[k][q][i].x : w[k][q][i].y, both = st & 1 ? __byte_perm(v, 0u, 0x4341) : v & 0x00ff00ffu, one = (st & 1 ? both : v) & 0x000f000fu;
-                            if (st == 0) ka_mma0(a[k][q][i], qa, one, both);
-                            else ka_mma(a[k][q][i], qa, one, both);
+                            const uint32_t v = st < 2 ? w[k][q][i].x : w[k][q][i].y, b0 = ka_codes(v, 2 * (st & 1)), b1 = ka_codes(v, 2 * (st & 1) + 1);
+                            if (st == 0) ka_mma0(a[k][q][i], qa, b0, b1);
+                            else ka_mma(a[k][q][i], qa, b0, b1);
                         }
                 }
             const uint2 qs = s.qsum[lane];
@@ -392,16 +405,20 @@ struct ka {
                 for (int i = 0; i < 2; ++i) { // lowest sum(q)
                     float d[4];
                     ka_mma0(d, make_uint4(qs.x, qs.y, 0u, 0u), pair[k][i], 0u);
-                    r[k].sc[2 * i] = (d[0] + d[2]) * 3.814697265625e-06f; // 2^-18: the codes' 2^-24 over the sums' 2^-6
-                    r[k].sc[2 * i + 1] = (d[1] + d[3]) * 3.814697265625e-06f;
+                    r[k].sc[2 * i] = (d[0] + d[2]) * 6.103515625e-05f; // 2^-14: the codes' 2^-20 over the sums' 2^-6
+                    r[k].sc[2 * i + 1] = (d[1] + d[3]) * 6.103515625e-05f;
                 }
 #pragma unroll
                 for (int q = 0; q < S; ++q) {
                     const uint4 pr = *reinterpret_cast<const uint4*>(blk + 16 * D + (q * 16 + 4 * ft) * 4);
-                    r[k].sc[0] = fmaf(ka_pair(pr.x).x, a[k][q][0][0] + a[k][q][0][2], r[k].sc[0]);
-                    r[k].sc[1] = fmaf(ka_pair(pr.y).x, a[k][q][0][1] + a[k][q][0][3], r[k].sc[1]);
-                    r[k].sc[2] = fmaf(ka_pair(pr.z).x, a[k][q][1][0] + a[k][q][1][2], r[k].sc[2]);
-                    r[k].sc[3] = fmaf(ka_pair(pr.w).x, a[k][q][1][1] + a[k][q][1][3], r[k].sc[3]);
+                    const float scale[4] = {ka_pair(pr.x).x, ka_pair(pr.y).x, ka_pair(pr.z).x, ka_pair(pr.w).x};
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 sum = ka_add2(make_float2(a[k][q][i][0], a[k][q][i][1]), make_float2(a[k][q][i][2], a[k][q][i][3]));
+                        const float2 sc = ka_fma2(make_float2(scale[2 * i], scale[2 * i + 1]), sum, make_float2(r[k].sc[2 * i], r[k].sc[2 * i + 1]));
+                        r[k].sc[2 * i] = sc.x;
+                        r[k].sc[2 * i + 1] = sc.y;
+                    }
                 }
                 if (!FULL) { // rows that the column does not see, or that are not there
                     const int lim = s.limit[g] - row0 - 16 * (warp + 8 * k);
@@ -489,23 +506,17 @@ struct ka {
                 ka_split_up(ka_mul2(w[k][0], make_float2(up, up)), pa.x, pa.y);
                 ka_split_up(ka_mul2(w[k][1], make_float2(up, up)), pa.z, pa.w);
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const uint32_t y = j < 4 ? a0 : a1, z = j < 4 ? c0 : c1;
-                    const uint32_t yb = j & 2 ? __byte_perm(y, 0u, 0x4341) : y & 0x00ff00ffu, zb = j & 2 ? __byte_perm(z, 0u, 0x4341) : z & 0x00ff00ffu;
-                    const uint32_t y1 = (j & 2 ? yb : y) & 0x000f000fu, z1 = (j & 2 ? zb : z) & 0x000f000fu;
-                    if (k == 0) {
-                        ka_mma0(d[j], pa, y1, z1);
-                        ka_mma0(d[j + 1], pa, yb, zb);
-                    } else {
-                        ka_mma(d[j], pa, y1, z1);
-                        ka_mma(d[j + 1], pa, yb, zb);
-                    }
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t y = ka_codes(j < 4 ? a0 : a1, j & 3), z = ka_codes(j < 4 ? c0 : c1, j & 3);
+                    if (k == 0) ka_mma0(d[j], pa, y, z);
+                    else ka_mma(d[j], pa, y, z);
                 }
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                acc[j][0] += fmaf(d[j][2], KA_REST, d[j][0]);
-                acc[j][1] += fmaf(d[j][3], KA_REST, d[j][1]);
+                const float2 sum = ka_add2(make_float2(acc[j][0], acc[j][1]), ka_fma2(make_float2(d[j][2], d[j][3]), make_float2(KA_REST, KA_REST), make_float2(d[j][0], d[j][1])));
+                acc[j][0] = sum.x;
+                acc[j][1] = sum.y;
             }
         }
         if (BW <= 2) lowest();
@@ -584,14 +595,14 @@ struct ka {
         if (2 * ft + 1 < S) s.part[warp][g][2 * ft + 1] = fmaf(low[3], KA_REST, low[1]);
         if (ft == 2) s.part[warp][g][S] = fmaf(low[2], KA_REST, low[0]);
         if (ft == 0 && warp == 0) s.m[g] = m;
-        const float even = room * ka_pow2(24 - KA_WEIGHT - KA_ROOM), odd = even * 0.0625f; // 2^24 / up
+        const float unit = room * ka_pow2(20 - KA_WEIGHT - KA_ROOM); // 2^20 / up
         __syncthreads(); // the probabilities have been read
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 8; j += 4)
                 *reinterpret_cast<float4*>(&s.sum[part][g][group * 64 + 8 * (2 * ft + i) + j]) =
-                    make_float4(acc[j][i] * even, (acc[j + 1][i] - acc[j][i]) * odd, acc[j + 2][i] * even, (acc[j + 3][i] - acc[j + 2][i]) * odd);
+                    make_float4(acc[j][i] * unit, acc[j + 1][i] * unit, acc[j + 2][i] * unit, acc[j + 3][i] * unit);
         __syncthreads();
         float* rec = p.records + ((size_t)blockIdx.x * 2 + (first ? 1 : 0)) * KA_COLS * LB_KV4_REC(D);
         for (int o = t; o < KA_COLS * D / 8; o += KA_THREADS) { // eight features a thread

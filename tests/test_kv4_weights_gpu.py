@@ -120,3 +120,22 @@ def test_normalised_queries_of_any_size(lb, ctx, dim, size, kind):
     case = kc.Case(ctx, dim, 2, 1, 512, seqs=[0], pos=[300], new=[2])
     attention(lb, ctx, case, 3, kind, norm=True, rot=32, size=size)
     case.free()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("length,size", [(2, 1.0), (30, 3.0), (1000, 3.0), (1000, 8.0), (5000, 1.0)])
+def test_two_terms(lb, ctx, dim, length, size):
+    """ordinary rows and queries, to the bits of two terms"""
+    case = kc.Case(ctx, dim, 2, 2, -(-length // 16) * 16, seqs=[1, 0], pos=[length - 1, length // 2], new=[1, 1])
+    rng, G = np.random.default_rng(7), 3
+    q = (size * rng.standard_normal((2, 2 * G, dim))).astype(np.float32)
+    d_q, out = ctx.to_device(q), ctx.alloc(q.size * 2)
+    ctx.kv4_attention(case.desc, case.batch, d_q, None, 0, 0, lb.IN_F32, None, out, 2 * G, 1, 0, 1e7, 1e-6)
+    got = out.download(np.float16).astype(np.float64).reshape(q.shape)
+    for row, seq, pos in case.places():
+        for h in range(2 * G):
+            want, tol = close(q[row, h].astype(np.float64), *kc.cache_rows(case.cache, dim, seq, h // G, pos + 1), pos)
+            assert (np.abs(got[row, h] - want) <= rounded(want, tol)).all(), (row, h)
+    for b in (d_q, out):
+        b.free()
+    case.free()
