@@ -139,3 +139,28 @@ def test_two_terms(lb, ctx, dim, length, size):
     for b in (d_q, out):
         b.free()
     case.free()
+
+
+@pytest.mark.parametrize("dim,heads,G", [(64, 2, 5), (128, 4, 4), (256, 2, 6)])
+def test_a_sequence_alone_and_in_any_batch(lb, ctx, dim, heads, G):
+    """where a batch cuts a sequence's rows depends on what else is in it, and so does the order of sums, but not the result beyond the bounds"""
+    pos, n = [4000, 10, 700, 2000, 3000, 55], 6
+    case = kc.Case(ctx, dim, heads, n, 4096, seqs=range(n), pos=pos, new=[1] * n)
+    HQ = heads * G
+    q = np.random.default_rng(8).standard_normal((n, HQ, dim)).astype(np.float32)
+    rows = [[kc.cache_rows(case.cache, dim, s, h, p + 1) for h in range(heads)] for s, p in enumerate(pos)]
+    bounds = [[close(q[s, h].astype(np.float64), *rows[s][h // G], pos[s]) for h in range(HQ)] for s in range(n)]
+    starts = ctx.to_device(np.arange(n + 1, dtype=np.int32))
+    for batch in ([0], [1], [2], [3], [4], [5], [0, 1, 2, 3, 4, 5], [5, 4, 3, 2, 1, 0], [3, 0, 5, 1], [0, 0, 4, 0]):
+        d = [ctx.to_device(np.array(a, np.int32)) for a in (batch, [pos[s] for s in batch])]
+        d_q, out = ctx.to_device(q[batch]), ctx.alloc(len(batch) * HQ * dim * 2)
+        call = lb.Kv4Batch(d[0].ptr, d[1].ptr, starts.ptr, len(batch), len(batch))
+        ctx.kv4_attention(case.desc, call, d_q, None, 0, 0, lb.IN_F32, None, out, HQ, 1, 0, 1e7, 1e-6)
+        got = out.download(np.float16).astype(np.float64).reshape(len(batch), HQ, dim)
+        for i, s in enumerate(batch):
+            for h in range(HQ):
+                assert (np.abs(got[i, h] - bounds[s][h][0]) <= rounded(*bounds[s][h])).all(), (batch, i, h)
+        for b in (*d, d_q, out):
+            b.free()
+    starts.free()
+    case.free()
