@@ -164,3 +164,18 @@ def test_a_sequence_alone_and_in_any_batch(lb, ctx, dim, heads, G):
             b.free()
     starts.free()
     case.free()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("gap", [12.0, 16.3, 18.3, 21.0])
+@pytest.mark.parametrize("length", [4096, 100001])
+def test_rows_exactly_alike_far_below_the_largest(lb, ctx, dim, length, gap):
+    """equal scores and scales, so that every row's weight is rounded to the same side: nothing averages out"""
+    case = rows_case(ctx, dim, length, 1, np.where(np.arange(length) == 0, 0.0, gap), np.where(np.arange(length) == 0, 0.0, 0.3), seed=dim, heads=1)
+    pairs = case.cache[1, :, :, 16 * dim:].copy().view(np.float16).reshape(1, -1, 2, dim // 64, 16, 2)
+    pairs[:, :, 0, :, :, 0] = 0
+    pairs[:, :, 1, :, :, 0], pairs[:, :, 1, :, :, 1] = 0.3, -2.25
+    pairs[:, 0, 1, :, 0] = 0
+    case.cache[1, :, :, 16 * dim:] = pairs.view(np.uint8).reshape(1, pairs.shape[1], -1)
+    case.d_cache.upload(case.cache)
+    check(lb, ctx, case, 1)
