@@ -323,7 +323,7 @@ int lb_kv4_attention(lb_ctx* ctx, const lb_kv4_cache* cache, const lb_kv4_batch*
  * draft where draft_probs = 0 (drafts that were not drawn).  Logits of -infinity or NaN have probability 0.
  *   Row by row a draft x stands while  u_accept[row] * q(x) < p(x)  (greedy: while it is the arg-max).  The first row that does not stand, or the last one, gives the token: the
  * first one, by index (top_k: by rank), at which the running sum of weights exceeds u_pick[r] times the whole, weights max(p - q, 0), at the last row p (and where the former are all
- * 0).  Probabilities and sums that choose the token are computed in 64 bits; the p that a draft is held against, over the whole vocabulary, to 2^-19 of itself.
+ * 0).  Probabilities and sums that choose the token are computed in 64 bits (exponentials of a whole row to 2^-42 of themselves); the p that a draft is held against, over the whole vocabulary, to 2^-19 of itself.
  * tokens i32 [rows]: the drafts that stand, the token, then -1; accepted i32 [n_reqs]: how many stand, -1 for a request without rows; p_out fp32 [rows] (0: not wanted):
  * p of every draft, 0 in last rows.  Rows behind the last request's are left as they were; a request that names rows that are not there gets -1, status word 0x1006. */
 enum { LB_VERIFY_MAX_REQS = 256, LB_VERIFY_MAX_ROWS = 8192 };

@@ -36,6 +36,6 @@ LB_API int lb_verify_drafts(lb_ctx* c, uint64_t logits, int vocab, uint64_t star
     unsigned cl = cluster_of(rows, vocab, 3 * c->sm_count);
     LB_TRY(lb_launch_cluster(c, kernel, (unsigned)rows, cl, 1, 512, 0, params, 1, cl));
     if (kernel != LBK_vd_rows) return lb_launch(c, LBK_vd_pick_short, (unsigned)n_reqs, 1, 1, 32, 0, params, 1);
-    cl = cluster_of(n_reqs, vocab, 2 * c->sm_count); /* one a time on an SM; requests take one pass or two, so that two waves even out: 48 requests 100 us as 6 CTAs each, 105 as 3 */
+    cl = cluster_of(n_reqs, vocab, 2 * c->sm_count); /* one a time on an SM; requests take one pass or two, so that two waves even out: 48 requests 88 us as 6 CTAs each, 90 as 3; but 30 requests 68 as 8 where 4 would take 62 */
     return lb_launch_cluster(c, LBK_vd_pick, (unsigned)n_reqs, cl, 1, 512, 0, params, 1, cl);
 }

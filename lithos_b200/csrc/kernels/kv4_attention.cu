@@ -9,26 +9,26 @@
 //     scores = sum over groups of scale_t (q . c_t) + lowest_t sum(q); read-out = sum of (p_t scale_t) c_t + p_t lowest_t.
 //   * q, p and p scale go in as two fp16 terms, the leading one in rows 0..7 of a product and what it leaves in rows 8..15: 22 bits of each, for the price of rows that eight
 //     columns would leave empty.  Weights are 2^9 at their reference and their second terms go in 2^11 up, so that the 22 bits reach down to 2^-23 of it; below that 2^-45 of
-//     it stays, which many rows far below one that has the top score and small values need.  A query is scaled by a power of two to [2^13, 2^14) at its largest.  Scores, sums and read-outs are fp32, a tile's read-outs added up
-//     by themselves (the products' own additions cut off); the output is fp16, what lb_gemm_int4 takes.
+//     it stays, which many rows far below one that has the top score and small values need.  A query is scaled by a power of two to [2^13, 2^14) at its largest.  Scores, sums and
+//     read-outs are fp32, a tile's read-outs added up by themselves (the products' own additions cut off); the output is fp16, what lb_gemm_int4 takes.
 //   * lowest_t sum(q) is one product more per 8 rows, p_t lowest_t and the sum of p one per 16.
 //   * A tile is 32768 / D rows, 36 KB, one bulk copy, requested by whichever warp is the last to be done with the place it goes to.  A warp does the scores of 256 / D blocks of
 //     16 rows and leaves their probabilities in shared memory; after a barrier it reads a group's 64 features out over its part of the tile, weights - probabilities times that
-//     group's scales, multiplied in 32 bits - as operands (44.4 us at 100 001 rows with the products written for all groups by whoever has the scores, 41 so).  References are standing:
+//     group's scales, multiplied in 32 bits - as operands (with the products written for all groups by whoever has the scores 100 001 rows took 8 % longer).  References are standing:
 //     probabilities are taken against the largest score, and a warp's weights of a column against the largest of them, at the last time that one passed its reference by 2^6, for
 //     which fp16 has room; so a tile usually costs one barrier and no exchange of maxima.  (A reference from the scales alone, 2 % faster, lost the bits of all rows
 //     that have weight where a row that has none is of large scale.)  Tiles whose rows are all there and seen by every column, most, take a path
-//     without those checks (46.6 -> 44.4).
+//     without those checks (5 %).
 //   * All tiles of all items are dealt evenly to the CTAs in one line, with places of one and a half tiles for an item's queries and results, so that ragged batches balance (32
-//     sequences: 74 us without such places, 61 with a tile's, 57 so); an item cut by a border leaves records that kv4_merge joins in order.
+//     sequences in an earlier kernel: 74 us without such places, 61 with a tile's, 57 so); an item cut by a border leaves records that kv4_merge joins in order.
 // mma.sync rather than tcgen05: the columns are few (6 for one token of 24 heads on 4), and codes would have to be widened into shared or tensor memory for it.
-// Bound by the latency of a tile's steps, with 16 warps an SM (as many as 128 registers leave) to hide it: per tile and SM some 610 instructions a warp (issue slots 44 %
-// busy), 180 passes through shared memory a warp (half of its time: queries 64, codes 32, copies in 36, scales 36, probabilities 20), the tensor pipe 38 %.
-// us a call with the merge, 24 / 4 heads of 256: one sequence of 4096 rows 11.1, of 100 001 41.3 (2.8 TB/s); 32 of 40 to 16 000 rows 52 (2.8 TB/s); 16 of 500 to 9001 rows with up
-// to 5 new tokens 73.8; 64 of 17 to 3001 rows, 32 / 8 heads of 128: 37.3 (39.5 where the parts of a tile were added up in turns at an item's end).  Tried without gain, us at 100 001 rows where 41 now or as given: warps of their own for scores and
-// read-outs (8 + 8 with the queries in registers 66, two CTAs of 6 + 2 60, both where 48); 16 columns at a time on half as many warps (150 where passes of eight took 118); three CTAs of
-// four warps with the queries in registers (54 where 48); maxima exchanged for every tile (52 where 48); barriers and references of the warps that share blocks alone (41.5);
-// a block's scales by shuffles (41.3); the next launch let in early (13.9 at 4096 rows where 12.4: its waiting CTAs are in the way).
+// Bound by the latency of a tile's steps, with 16 warps an SM (as many as 128 registers leave) to hide it: per tile and SM some 720 instructions a warp (issue slots 48 %
+// busy), 180 passes through shared memory a warp (half of its time: queries 64, codes 32, copies in 36, scales 36, probabilities 20), the tensor pipe 34 %.
+// us a call with the merge, 24 / 4 heads of 256: one sequence of 4096 rows 11.2, of 100 001 43.9 (2.6 TB/s); 32 of 40 to 16 000 rows 54.4 (2.6 TB/s); 16 of 500 to 9001 rows with up
+// to 5 new tokens 79.3; 64 of 17 to 3001 rows, 32 / 8 heads of 128: 38.5, of 64: 31.  Tried without gain, with the time of the kernel of then: warps of their own for scores and
+// read-outs (8 + 8 with the queries in registers 66 us at 100 001 rows, two CTAs of 6 + 2 60, both where 48); 16 columns at a time on half as many warps (150 where passes of eight took
+// 118); three CTAs of four warps with the queries in registers (54 where 48); maxima exchanged for every tile (52 where 48); barriers and references of the warps that share blocks
+// alone (41.5 where 41.0); a block's scales by shuffles (41.3 where 41.0); the next launch let in early (13.9 at 4096 rows where 12.4: its waiting CTAs are in the way).
 #include "kv4.cuh"
 
 #define KA_WARPS 8

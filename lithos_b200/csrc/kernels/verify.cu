@@ -2,7 +2,7 @@
 //   p = softmax(logits / T) over the whole vocabulary or the top_k largest, q the draft's probabilities (or 1 at the draft).
 //   Draft x of a row stands while  u q(x) < p(x).  The first row of a request that does not stand, or its last row, which has no draft, gives the token: the
 //   first one whose cumulative weight exceeds u' times their sum, the weights being max(p - q, 0) (at the last row p).
-// What a token's choice depends on is computed in 64 bits: a border between two of 250 000 tokens lies within 2^-24 of some number often enough that 32 bits would pick a neighbour
+// What a token's choice depends on is computed in 64 bits (exponentials of a whole row to 2^-42): a border between two of 250 000 tokens lies within 2^-24 of some number often enough that 32 bits would pick a neighbour
 // in one draw of a hundred.  Whether a draft stands has a single border; there the sum of a row is one of 32-bit exponentials, four to a 64-bit addition.  Where logits x
 // under the maximum in log2 units carry it, it is off by 2^-22 for the exponential, 2^-24.5 x for its argument's factor and up to 2^-20.5 (x < 32) for the argument: 2^-19 of itself at most.
 // Two launches: every row by a cluster of up to 8 CTAs, then every request.  The first reads the logits once and is bound by that where there are many rows (5 TB/s at 188 rows of
