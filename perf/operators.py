@@ -167,6 +167,7 @@ def prepare(case, seed):
         state["b"]["k"], state["b"]["v"] = Buffer(t["kv"][:, :half]), Buffer(t["kv"][:, half:])
     if case.get("gate") and "q" in t:
         state["b"]["gate"] = Buffer(t["q"][:, :, case["D"]:])
+    torch.cuda.synchronize()  # the library's calls go to a stream of its own, which waits for no other
     return state
 
 
